@@ -335,6 +335,33 @@ LTX_API int ltx_attention(ltx_ctx* ctx, const void* q, int ldq, const void* k,
                           const void* gate_logits, int ldg, int tq, int tk,
                           int heads, int head_dim, void* stream);
 
+/* ---- the caption language model ------------------------------------------
+ * Attention operators of a decoder-only language model, as the captions'
+ * text encoder runs it beside the DiT (src/ltx25-text-encoder.cc; the
+ * reference leaves these to vpipe).  bf16 device tensors, token-major with
+ * head h at columns [h*D, (h+1)*D), row strides in elements (multiples of
+ * 8), 16-byte aligned; query head h reads key/value head
+ * h / (heads / kv_heads); head_dim 64, 128 or 256; at most 128 query heads a
+ * key/value head.  Sequence offsets, lengths and page tables are DEVICE
+ * int32 arrays: the host does not read them, the kernels bound every value by
+ * the sizes given here. */
+
+/* Attention over packed prompts of different lengths.  Sequence s has the
+ * query rows [cu_q[s], cu_q[s+1]) of q and o (`rows` rows) and the keys
+ * [cu_k[s], cu_k[s+1]) of k and v (`keys` rows); cu_q and cu_k have seqs + 1
+ * entries and do not descend.  Row i of n queries over m keys stands at
+ * position m - n + i; with causal != 0 it sees the keys j <= its position,
+ * with window > 0 only those above position - window:
+ *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j),
+ * zero where it sees none.  What lies outside a row's keys does not reach it,
+ * whatever it holds (NaN and infinities too).  Rows outside the sequences are
+ * left as they are.  o must not overlap q, k or v.  Allocates nothing. */
+LTX_API int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const void* k, int ldk,
+                                 const void* v, int ldv, void* o, int ldo, const int32_t* cu_q,
+                                 const int32_t* cu_k, int seqs, int rows, int keys, int heads,
+                                 int kv_heads, int head_dim, int causal, int window, float scale,
+                                 void* stream);
+
 /* ---- RoPE tables (host, once per generation) ----------------------------
  * The reference's build_rope / video_spans / audio_time_seconds
  * (src/ltx25-rope.cc:74-296), computed on the host into caller buffers; no

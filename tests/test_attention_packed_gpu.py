@@ -1,0 +1,232 @@
+"""Attention over packed prompts against its formula in 64 bits: ragged and empty
+sequences, rows that see nothing, grouped heads, windows, cached prefixes, head
+widths 64 / 128 / 256, NaN and infinities wherever a row does not look, strides,
+streams, captured graphs and refusals.  The bound is lm_ref's."""
+import math
+
+import pytest
+
+import lm_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def make(lens_q, lens_k, heads, kv_heads, D, seed=0, qscale=1.0, pad=0):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    cu_q, cu_k = lm_ref.offsets(lens_q), lm_ref.offsets(lens_k)
+    q = (torch.randn((cu_q[-1] + pad, heads * D), generator=g, device="cuda") * qscale)
+    kv = torch.randn((cu_k[-1] + pad, 2 * kv_heads * D), generator=g, device="cuda")
+    kv = kv.to(torch.bfloat16)
+    return q.to(torch.bfloat16), kv[:, :kv_heads * D], kv[:, kv_heads * D:], cu_q, cu_k
+
+
+def dev(cu):
+    import torch
+    return torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+
+def check(got, want, tol, cu_q):
+    import torch
+    a, b = cu_q[0], cu_q[-1]
+    got, want, tol = got[a:b].double(), want[a:b], tol[a:b]
+    assert torch.isfinite(got).all()
+    over = (got - want).abs() - tol
+    worst = float(over.max()) if over.numel() else 0.0
+    assert worst <= 1e-30, (worst, (over > 0).nonzero()[:5].tolist())
+
+
+CASES = [
+    # lens_q, lens_k, heads, kv_heads, D, causal, window, qscale
+    ([1], [1], 1, 1, 64, True, 0, 1.0),
+    ([1], [1], 4, 4, 128, True, 0, 1.0),
+    ([1], [1], 2, 1, 256, True, 0, 1.0),
+    ([256], [256], 32, 8, 128, True, 0, 1.0),
+    ([1, 2, 127, 128, 129, 1, 64, 255], None, 8, 2, 128, True, 0, 1.0),
+    ([1, 2, 127, 128, 129, 1, 64, 255], None, 4, 4, 64, True, 0, 1.0),
+    ([1, 2, 127, 128, 129, 1, 64, 257], None, 4, 1, 256, True, 0, 1.0),
+    ([0, 5, 0, 300, 0], None, 4, 2, 128, True, 0, 1.0),
+    ([0, 5, 0, 300, 0], [7, 5, 0, 400, 3], 4, 2, 64, False, 0, 1.0),
+    ([10, 200, 3], [3, 0, 1], 4, 2, 128, True, 0, 1.0),        # rows that see nothing
+    ([10, 200, 3], [3, 0, 1], 4, 2, 256, True, 0, 1.0),
+    ([10, 200, 3], [3, 0, 1], 4, 2, 64, True, 2, 1.0),
+    ([10, 5], [0, 0], 2, 2, 128, True, 0, 1.0),                # no keys at all
+    ([1, 60, 129], [1000, 333, 1029], 6, 2, 128, True, 0, 1.0),  # after a prefix
+    ([1, 60, 129], [1000, 333, 1029], 5, 1, 256, True, 0, 1.0),
+    ([1, 60, 129], [1000, 333, 1029], 14, 2, 64, True, 100, 1.0),
+    ([700], None, 7, 1, 128, True, 0, 1.0),
+    ([300, 90], None, 64, 1, 64, True, 0, 1.0),
+    ([40, 3], None, 128, 1, 64, True, 0, 1.0),
+    ([40, 3], None, 127, 1, 128, True, 0, 1.0),
+    ([500], None, 4, 2, 128, False, 0, 1.0),
+    ([500, 77], [130, 900], 4, 2, 256, False, 0, 1.0),
+    ([1000], None, 2, 2, 128, True, 1, 1.0),                   # itself alone
+    ([1000], None, 2, 2, 128, True, 128, 1.0),
+    ([1000, 444], None, 4, 2, 256, True, 300, 1.0),
+    ([1000, 444], None, 4, 2, 64, False, 300, 1.0),
+    ([1000], None, 2, 2, 64, True, 2147483647, 1.0),
+    ([1500], None, 2, 2, 128, True, 0, 6.0),                   # maxima that grow
+    ([1500], None, 2, 1, 64, False, 0, 6.0),
+    ([900], None, 2, 1, 256, True, 0, 6.0),
+    ([4099], None, 4, 1, 128, True, 0, 1.0),
+    ([2500], None, 2, 2, 256, True, 1024, 1.0),
+]
+
+
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv_heads,D,causal,window,qscale", CASES)
+def test_packed_attention_matches_64_bits(ctx, lens_q, lens_k, heads, kv_heads, D, causal, window,
+                                          qscale):
+    import torch
+    import ltx25_b200 as L
+    lens_k = lens_q if lens_k is None else lens_k
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, sum(lens_q) + D, qscale)
+    got = L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D,
+                             causal=causal, window=window)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, causal, window,
+                                        D ** -0.5)
+    check(got, want, tol, cu_q)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_outside_the_sequences_are_left_alone(ctx, D, causal):
+    """Rows before the first and behind the last sequence hold NaN and infinities
+    and are neither read into a result nor written."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads, first = 4, 2, 3
+    lens = [5, 130, 61]
+    q, k, v, _, _ = make(lens, lens, heads, kv_heads, D, 5, pad=80)
+    cu = lm_ref.offsets(lens, first)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=torch.bfloat16)
+    for x in (q, k, v):
+        x[:first] = bad[0]
+        x[cu[-1]:] = bad[torch.arange(x.shape[0] - cu[-1], device="cuda") % 3][:, None]
+    out = torch.full((q.shape[0], heads * D), 7.0, device="cuda", dtype=torch.bfloat16)
+    L.attention_packed(ctx, q, k, v, dev(cu), dev(cu), heads, kv_heads, D, causal=causal, out=out)
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.all(out[:first] == 7.0) and torch.all(out[cu[-1]:] == 7.0)
+    want, tol = lm_ref.attention_packed(q, k, v, cu, cu, heads, kv_heads, D, causal, 0, D ** -0.5)
+    check(out, want, tol, cu)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_a_row_does_not_see_does_not_reach_it(ctx, D, value):
+    """NaN and infinities in the keys and values of a neighbour sequence, and of
+    later tokens of the row's own."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads = 4, 2
+    lens = [70, 90, 200]
+    q, k, v, cu, _ = make(lens, lens, heads, kv_heads, D, 11)
+    k[cu[1]:cu[2]] = value                   # the whole second sequence
+    v[cu[1]:cu[2]] = value
+    spot = cu[2] + 150                       # one token of the third: a few dims
+    v[spot, 3:9] = value
+    got = L.attention_packed(ctx, q, k, v, dev(cu), dev(cu), heads, kv_heads, D)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu, cu, heads, kv_heads, D, True, 0, D ** -0.5)
+    for a, b in ((cu[0], cu[1]), (cu[2], spot)):
+        over = (got[a:b].double() - want[a:b]).abs() - tol[a:b]
+        assert torch.isfinite(got[a:b]).all()
+        assert float(over.max()) <= 0
+    # rows that do see it: the formula's own NaN or infinity, and only there
+    seen, ref = got[spot:cu[3]].double(), want[spot:cu[3]]
+    assert torch.equal(torch.isfinite(seen), torch.isfinite(ref))
+    ok = torch.isfinite(ref)
+    assert float(((seen - ref).abs() - tol[spot:cu[3]])[ok].max()) <= 0
+    assert torch.equal(seen[~ok].isnan(), ref[~ok].isnan())
+
+
+def test_rows_of_one_projection_and_other_streams(ctx):
+    """q, k and v as column slices of one buffer, on a stream of the caller's."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads, D = 8, 2, 64
+    lens = [33, 200]
+    cu = lm_ref.offsets(lens)
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        qkv = torch.randn((cu[-1], (heads + 2 * kv_heads) * D), device="cuda").to(torch.bfloat16)
+        c = dev(cu)
+    q = qkv[:, :heads * D]
+    k, v = qkv[:, heads * D:(heads + kv_heads) * D], qkv[:, (heads + kv_heads) * D:]
+    got = L.attention_packed(ctx, q, k, v, c, c, heads, kv_heads, D, stream=st)
+    st.synchronize()
+    want, tol = lm_ref.attention_packed(q, k, v, cu, cu, heads, kv_heads, D, True, 0, D ** -0.5)
+    check(got, want, tol, cu)
+
+
+def test_captured_and_replayed_with_new_lengths(ctx):
+    """One graph, replayed after the offsets changed on the device."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads, D = 4, 1, 128
+    q, k, v, _, _ = make([300], [300], heads, kv_heads, D, 3)
+    c = dev([0, 100, 300])
+    out = torch.zeros_like(q)
+    L.attention_packed(ctx, q, k, v, c, c, heads, kv_heads, D, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        L.attention_packed(ctx, q, k, v, c, c, heads, kv_heads, D, out=out)
+    for cu in ([0, 100, 300], [0, 1, 299], [17, 17, 230]):
+        c.copy_(dev(cu))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        ctx.check()
+        want, tol = lm_ref.attention_packed(q, k, v, cu, cu, heads, kv_heads, D, True, 0, D ** -0.5)
+        check(out, want, tol, cu)
+        assert torch.all(out[:cu[0]] == 7.0) and torch.all(out[cu[-1]:] == 7.0)
+
+
+def test_the_same_call_gives_the_same_bits(ctx):
+    import torch
+    import ltx25_b200 as L
+    lens = [411, 5, 900]
+    q, k, v, cu, _ = make(lens, lens, 8, 2, 128, 9)
+    a = L.attention_packed(ctx, q, k, v, dev(cu), dev(cu), 8, 2, 128)
+    b = L.attention_packed(ctx, q, k, v, dev(cu), dev(cu), 8, 2, 128)
+    assert torch.equal(a, b)
+
+
+def test_refusals(ctx):
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu, _ = make([20], [20], 4, 2, 64)
+    c = dev(cu)
+
+    def code(fn):
+        with pytest.raises(L.LtxError) as e:
+            fn()
+        return e.value.code
+
+    call = lambda **kw: L.attention_packed(ctx, **{**dict(                  # noqa: E731
+        q=q, k=k, v=v, cu_q=c, cu_k=c, heads=4, kv_heads=2, head_dim=64), **kw})
+    assert code(lambda: call(window=-1)) == -2
+    assert code(lambda: call(scale=0.0)) == -2
+    assert code(lambda: call(scale=math.nan)) == -2
+    assert code(lambda: call(scale=math.inf)) == -2
+    assert code(lambda: call(heads=4, kv_heads=3)) == -2
+    assert code(lambda: call(q=q.float())) == -3
+    assert code(lambda: call(q=q[:1].expand(20, -1))) == -2               # broadcast rows
+    assert code(lambda: call(cu_q=c.long())) == -2
+    assert code(lambda: call(cu_k=dev([0, 10, 20]))) == -2
+    assert code(lambda: call(q=q.cpu())) == -2
+    assert code(lambda: call(out=q[:10])) == -2
+    wide = torch.zeros((20, 4 * 64 + 4), device="cuda", dtype=torch.bfloat16)
+    assert code(lambda: call(q=wide[:, 1:257])) == -8
+    assert code(lambda: call(q=wide[:, :256])) == -8
+    w96 = torch.zeros((20, 96), device="cuda", dtype=torch.bfloat16)
+    assert code(lambda: call(q=w96, k=w96, v=w96, heads=1, kv_heads=1, head_dim=96)) == -2
+    none = L.attention_packed(ctx, q[:0], k, v, c, c, 4, 2, 64)            # nothing to do
+    assert none.shape == (0, 256)
+    torch.cuda.synchronize()
+    ctx.check()

@@ -127,4 +127,20 @@ int launch_sage_tc(const __nv_bfloat16* q, int ldq, const __nv_bfloat16* k, int 
                    __nv_bfloat16* o, int ldo, const __nv_bfloat16* gate, int ldg, int tq,
                    int tk, int heads, int head_dim, int* err, cudaStream_t s);
 
+// Attention over packed prompts (attention_packed.cu): bf16, token-major with
+// row strides ld* (elements, % 8 == 0, 16-byte aligned pointers); query head h
+// reads key/value head h / (heads / kv_heads).  cu_q, cu_k: device int32
+// [seqs + 1].  head_dim 64, 128 or 256, at most 128 query heads a key head.
+struct PackedAttention {
+  const __nv_bfloat16 *q = nullptr, *k = nullptr, *v = nullptr;
+  __nv_bfloat16* o = nullptr;
+  int ldq = 0, ldk = 0, ldv = 0, ldo = 0;
+  const int *cu_q = nullptr, *cu_k = nullptr;
+  int seqs = 0, rows = 0, keys = 0;   // rows of q and o, rows of k and v
+  int heads = 0, kv_heads = 0, head_dim = 0;
+  int causal = 1, window = 0;
+  float scale = 0.0f;
+};
+int launch_attention_packed(const PackedAttention& a, int* err, cudaStream_t s);
+
 }  // namespace ltx

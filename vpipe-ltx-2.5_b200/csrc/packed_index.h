@@ -1,0 +1,47 @@
+// packed_index.h -- where things are in packed sequences: row tiles, the keys
+// a row sees, cache pages.  Plain integer code without CUDA types, shared by
+// the kernels and compiled on its own by the CPU tests.
+//
+// Sequence s of a packed tensor has rows [cu[s], cu[s + 1]).  cu is device
+// data that no host code has looked at: every value goes through
+// clamp_int(cu, 0, rows) before it is used, so that a wrong one costs rows,
+// never an access out of bounds.
+#pragma once
+
+#if defined(__CUDACC__)
+#define LTX_HD __host__ __device__ __forceinline__
+#else
+#define LTX_HD inline
+#endif
+
+namespace ltx {
+
+LTX_HD int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+// Work slots of a tensor of `rows` packed rows: sequence s owns the slots from
+// slot_base(cu[s], s) up to slot_base(cu[s + 1], s + 1), computed from its own
+// offset alone (no prefix sum over the sequences before it).  A sequence of n
+// rows gets at least n / tile + extra - 1 slots, rounded up:
+//   floor((a + n) / t) + x - floor(a / t)  >=  floor(n / t) + x.
+// extra 1 covers ceil(n / t) row tiles; extra 2 covers the tiles of a run that
+// starts anywhere inside a tile (ceil(n / t) + 1 of them for n > 0, and one
+// where n < 2).  Slots past a sequence's last tile are empty.
+LTX_HD int slot_base(int start, int seq, int tile, int extra) { return start / tile + extra * seq; }
+LTX_HD int slot_count(int rows, int seqs, int tile, int extra)
+{
+  return slot_base(rows, seqs, tile, extra);
+}
+
+// Row i of n rows over m keys stands at position m - n + i.
+// The keys it sees are [key_low, key_high).
+LTX_HD int key_high(int pos, int m, int causal)
+{
+  if (!causal) return m;
+  return pos < 0 ? 0 : (pos < m ? pos + 1 : m);
+}
+LTX_HD int key_low(int pos, int window)
+{
+  return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
+
+}  // namespace ltx

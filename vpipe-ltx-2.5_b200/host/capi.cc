@@ -16,6 +16,7 @@
 #include "ltx25-cuda-ops.h"
 #include "ltx25-adaln.h"
 #include "ltx25-connector-cuda.h"
+#include "ltx25-lm-ops.h"
 #include "ltx25-safetensors.h"
 
 struct ltx_ctx {
@@ -686,6 +687,45 @@ int ltx_attention(ltx_ctx* ctx, const void* q, int ldq, const void* k, int ldk,
                             static_cast<const __nv_bfloat16*>(gate_logits), ldg, tq, tk,
                             heads, head_dim, &e, /*layer*/ 1 << 30))
       return fail(ctx, code_for(e), e);
+    return LTX_OK;
+  });
+}
+
+int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const void* k, int ldk,
+                         const void* v, int ldv, void* o, int ldo, const int32_t* cu_q,
+                         const int32_t* cu_k, int seqs, int rows, int keys, int heads,
+                         int kv_heads, int head_dim, int causal, int window, float scale,
+                         void* stream)
+{
+  return guarded([&]() -> int {
+    OnDevice on_(dev_of(ctx));
+    if (ctx == nullptr) return LTX_E_NULL;
+    ltx::PackedAttention a;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.k = static_cast<const __nv_bfloat16*>(k);
+    a.v = static_cast<const __nv_bfloat16*>(v);
+    a.o = static_cast<__nv_bfloat16*>(o);
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldo = ldo;
+    a.cu_q = cu_q;
+    a.cu_k = cu_k;
+    a.seqs = seqs;
+    a.rows = rows;
+    a.keys = keys;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.causal = causal != 0;
+    a.window = window;
+    a.scale = scale;
+    std::string e;
+    const int rc = ltx25::check_attention_packed(a, &e);
+    if (rc != LTX_OK) return fail(ctx, rc, e);
+    if (seqs == 0 || rows == 0) return LTX_OK;
+    if (ltx::launch_attention_packed(a, ctx->ops.err_word(), S(stream)) != 0)
+      return fail(ctx, LTX_E_CUDA, "attention_packed launch failed");
     return LTX_OK;
   });
 }

@@ -1,0 +1,97 @@
+// ltx25-lm-ops.cc -- argument checks of the language-model operators.
+#include "ltx25-lm-ops.h"
+
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/ltx25_cuda.h"
+
+namespace ltx25 {
+
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// heads, head width and the factor of the scores
+int check_heads(const char* op, int heads, int kv_heads, int head_dim, int window, float scale,
+                std::string* why)
+{
+  const std::string o(op);
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > 128) {
+    *why = o + ": need heads a multiple of kv_heads, at most 128 heads a kv head";
+    return LTX_E_SHAPE;
+  }
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+    *why = o + ": need head_dim 64, 128 or 256";
+    return LTX_E_SHAPE;
+  }
+  if (window < 0) {
+    *why = o + ": need window >= 0 (0: no window)";
+    return LTX_E_SHAPE;
+  }
+  if (!(scale > 0.0f) || !std::isfinite(scale)) {
+    *why = o + ": need a finite scale > 0";
+    return LTX_E_SHAPE;
+  }
+  return LTX_OK;
+}
+
+// a bf16 operand of `rows` rows of `cols` elements
+int check_rows(const char* op, const char* name, const void* p, int ld, int rows, long long cols,
+               std::string* why)
+{
+  if (rows == 0) return LTX_OK;
+  const std::string o = std::string(op) + ": " + name;
+  if (p == nullptr) {
+    *why = o + " is null";
+    return LTX_E_NULL;
+  }
+  if (!aligned(p, 16) || ld % 8 != 0) {
+    *why = o + " must be 16-byte aligned with a row stride % 8 == 0";
+    return LTX_E_ALIGN;
+  }
+  if (ld < cols) {
+    *why = o + ": need a row stride of at least heads * head_dim";
+    return LTX_E_SHAPE;
+  }
+  return LTX_OK;
+}
+
+int check_ints(const char* op, const char* name, const int* p, std::string* why)
+{
+  const std::string o = std::string(op) + ": " + name;
+  if (p == nullptr) {
+    *why = o + " is null";
+    return LTX_E_NULL;
+  }
+  if (!aligned(p, 4)) {
+    *why = o + " must be 4-byte aligned";
+    return LTX_E_ALIGN;
+  }
+  return LTX_OK;
+}
+
+}  // namespace
+
+int check_attention_packed(const ltx::PackedAttention& a, std::string* why)
+{
+  const char* op = "attention_packed";
+  int rc = check_heads(op, a.heads, a.kv_heads, a.head_dim, a.window, a.scale, why);
+  if (rc != LTX_OK) return rc;
+  if (a.seqs < 0 || a.rows < 0 || a.keys < 0) {
+    *why = "attention_packed: need seqs, rows and keys >= 0";
+    return LTX_E_SHAPE;
+  }
+  if (a.seqs == 0 || a.rows == 0) return LTX_OK;
+  const long long qc = (long long)a.heads * a.head_dim, kc = (long long)a.kv_heads * a.head_dim;
+  if ((rc = check_ints(op, "cu_q", a.cu_q, why)) != LTX_OK ||
+      (rc = check_ints(op, "cu_k", a.cu_k, why)) != LTX_OK ||
+      (rc = check_rows(op, "q", a.q, a.ldq, a.rows, qc, why)) != LTX_OK ||
+      (rc = check_rows(op, "o", a.o, a.ldo, a.rows, qc, why)) != LTX_OK ||
+      (rc = check_rows(op, "k", a.k, a.ldk, a.keys, kc, why)) != LTX_OK ||
+      (rc = check_rows(op, "v", a.v, a.ldv, a.keys, kc, why)) != LTX_OK)
+    return rc;
+  return LTX_OK;
+}
+
+}  // namespace ltx25

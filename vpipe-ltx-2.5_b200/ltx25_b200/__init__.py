@@ -104,6 +104,8 @@ SIGNATURES = {
     "ltx_qk_norm_rope": (_I, [_P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P]),
     "ltx_attention": (_I, [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I,
                            _I, _I, _P]),
+    "ltx_attention_packed": (_I, [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P, _P] + [_I] * 8
+                             + [ctypes.c_float, _P]),
     "ltx_block_create": (_I, [_P, _I, _I, _I, _I, ctypes.POINTER(_P)]),
     "ltx_block_destroy": (None, [_P]),
     "ltx_block_last_error": (ctypes.c_char_p, [_P]),
@@ -746,6 +748,84 @@ def attention(ctx, q, k, v, heads, head_dim, gate=None, tq=None, tk=None,
         0 if gate is None else gate.stride(0), tq, tk, heads, head_dim,
         _stream(stream)), "attention")
     return o
+
+
+# ---- the caption language model -------------------------------------------------
+
+
+def _stream_of(ctx, stream):
+    """The stream handle of a call on `ctx`: the current stream of the context's
+    device unless one is given."""
+    if stream is None:
+        import torch
+        return ctypes.c_void_p(torch.cuda.current_stream(ctx.device).cuda_stream)
+    return _stream(stream)
+
+
+def _new_on(ctx, stream, make):
+    """make() with allocations ordered on the call's stream."""
+    import torch
+    if stream is None:
+        return make()
+    s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+    with torch.cuda.stream(s):
+        return make()
+
+
+def _need(ok, code, what):
+    if not ok:
+        raise LtxError(code, what)
+
+
+def _rows(ctx, t, cols, name):
+    """A [rows][cols] bf16 tensor on the context's device with adjacent columns."""
+    import torch
+    _need(t.dtype == torch.bfloat16, -3, f"{name}: need bfloat16, got {t.dtype}")
+    _need(t.dim() == 2 and t.shape[1] == cols and (t.stride(1) == 1 or t.shape[0] == 0), -2,
+          f"{name}: need [rows][{cols}] with adjacent columns, got {tuple(t.shape)}")
+    _need(t.device.type == "cuda" and t.device.index == ctx.device, -2,
+          f"{name}: need a tensor on cuda:{ctx.device}, got {t.device}")
+    # one row (or none) has no stride to speak of; a broadcast one stays as it is,
+    # and is refused
+    return t.stride(0) if t.shape[0] > 1 else (cols + 7) // 8 * 8
+
+
+def _ints(ctx, t, n, name):
+    """A contiguous int32 tensor of n values on the context's device."""
+    import torch
+    _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n, -2,
+          f"{name}: need {n} adjacent int32 values, got {tuple(t.shape)} {t.dtype}")
+    _need(t.device.type == "cuda" and t.device.index == ctx.device, -2,
+          f"{name}: need a tensor on cuda:{ctx.device}, got {t.device}")
+    return _ptr(t)
+
+
+def attention_packed(ctx, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal=True, window=0,
+                     scale=None, out=None, stream=None):
+    """ltx_attention_packed: attention of packed sequences, q [rows][heads * D],
+    k and v [keys][kv_heads * D] bf16 (column slices of one projection's output
+    are fine), cu_q and cu_k int32 [seqs + 1] on the device.  scale: 1/sqrt(D) by
+    default.  Returns [rows][heads * D]; rows outside the sequences are left as
+    they are in `out`."""
+    import torch
+    seqs = cu_q.numel() - 1
+    ldq = _rows(ctx, q, heads * head_dim, "q")
+    ldk = _rows(ctx, k, kv_heads * head_dim, "k")
+    ldv = _rows(ctx, v, kv_heads * head_dim, "v")
+    _need(k.shape[0] == v.shape[0], -2, "attention_packed: k and v differ in rows")
+    pq, pk = _ints(ctx, cu_q, seqs + 1, "cu_q"), _ints(ctx, cu_k, seqs + 1, "cu_k")
+    rows = q.shape[0]
+    if out is None:
+        out = _new_on(ctx, stream, lambda: torch.empty((rows, heads * head_dim), dtype=q.dtype,
+                                                       device=q.device))
+    ldo = _rows(ctx, out, heads * head_dim, "out")
+    _need(out.shape[0] == rows, -2, "attention_packed: out and q differ in rows")
+    ctx._ok(ctx.lib.ltx_attention_packed(
+        ctx.h, _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out), ldo, pq, pk, seqs, rows,
+        k.shape[0], heads, kv_heads, head_dim, int(causal), window,
+        head_dim ** -0.5 if scale is None else scale, _stream_of(ctx, stream)),
+        "attention_packed")
+    return out
 
 
 def is_quantized_name(name, ndim):
