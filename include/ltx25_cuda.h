@@ -362,6 +362,66 @@ LTX_API int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const voi
                                  int kv_heads, int head_dim, int causal, int window, float scale,
                                  void* stream);
 
+/* An 8-bit key/value cache: pages of LTX_KV8_PAGE tokens in the caller's
+ * device memory.  Codes are int8 [pages][kv_heads][LTX_KV8_PAGE][head_dim],
+ * with one bf16 scale for each page and head ([pages][kv_heads]), keys and
+ * values each; a code c stands for c * scale.  Token t of sequence s is slot
+ * t % LTX_KV8_PAGE of page table[s][t / LTX_KV8_PAGE] (table_ld columns).  A
+ * page's content needs no clearing before its first use.  Sequences may share
+ * pages that nothing is appended to.
+ *
+ * A start, length or page outside the cache is not followed: the rows or
+ * tokens that need it are left out, and the next ltx_ctx_check returns
+ * LTX_E_KERNEL. */
+#define LTX_KV8_PAGE 64
+typedef struct {
+  int8_t* k;
+  int8_t* v;
+  uint16_t* k_scale;
+  uint16_t* v_scale;
+  int pages;
+  int kv_heads;
+  int head_dim;
+} ltx_kv8_cache;
+
+/* Appends bf16 keys and values: row cu[s] + i of k and v (`rows` rows,
+ * [kv_heads * head_dim] columns) becomes token starts[s] + i of sequence s.
+ * Each page and head that gets tokens takes as scale the smallest bf16 with
+ * 127 * scale >= |x| for the new values, or keeps its own where that is
+ * larger and the page holds tokens of the sequence already
+ * (starts[s] % LTX_KV8_PAGE != 0, first page).  New codes are
+ * rint(x / scale); codes the page held are brought to a grown scale as
+ * rint(code * old / new).  A NaN or infinity makes the scale of its page and
+ * head NaN.  The pages that get tokens belong to one sequence each. */
+LTX_API int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,
+                           const void* v, int ldv, const int32_t* cu, const int32_t* starts,
+                           const int32_t* table, int table_ld, int seqs, int rows, void* stream);
+
+/* The reverse: tokens starts[s] + i as bf16(code * scale) into row cu[s] + i of
+ * k and v, as ltx_attention_packed takes them (a prompt's next chunk over what
+ * the cache holds). */
+LTX_API int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int ldk, void* v,
+                         int ldv, const int32_t* cu, const int32_t* starts, const int32_t* table,
+                         int table_ld, int seqs, int rows, void* stream);
+
+/* Attention of new tokens over the cache: rows [cu_q[s], cu_q[s+1]) of q and o
+ * are the last tokens of sequence s, whose lengths[s] tokens (those included)
+ * the cache holds; row i of n sees the tokens up to its own position
+ * lengths[s] - n + i, with window > 0 only those above position - window.  The
+ * result is ltx_attention_packed's over the values the codes stand for.  One
+ * token a sequence is the usual call; the cache is read once for each 16 rows
+ * (tokens times the query heads of a key/value head).  max_len sizes the
+ * launch: the largest length expected.  The workspace is the caller's,
+ * ltx_kv8_attention_workspace bytes whatever the lengths, 16-byte aligned; two
+ * calls that may run at once (streams, captured graphs) need one each.
+ * Allocates nothing. */
+LTX_API int ltx_kv8_attention_workspace(ltx_ctx* ctx, int head_dim, size_t* bytes);
+LTX_API int ltx_kv8_attention(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* q, int ldq,
+                              void* o, int ldo, const int32_t* cu_q, const int32_t* lengths,
+                              const int32_t* table, int table_ld, int seqs, int rows, int heads,
+                              int max_len, int window, float scale, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ---- RoPE tables (host, once per generation) ----------------------------
  * The reference's build_rope / video_spans / audio_time_seconds
  * (src/ltx25-rope.cc:74-296), computed on the host into caller buffers; no

@@ -17,6 +17,16 @@ int t_base(int a, int s, int t, int x) { return ltx::slot_base(a, s, t, x); }
 int t_count(int r, int s, int t, int x) { return ltx::slot_count(r, s, t, x); }
 int t_high(int p, int m, int c) { return ltx::key_high(p, m, c); }
 int t_low(int p, int w) { return ltx::key_low(p, w); }
+int t_span_ok(int s, int n, int c) { return ltx::span_ok(s, n, c); }
+int t_page_ok(int g, int n) { return ltx::page_ok(g, n); }
+void t_span(int s, int n, int i, int* o) {
+  const ltx::PageSpan r = ltx::page_span(s, n, i);
+  o[0] = r.block; o[1] = r.a; o[2] = r.b;
+}
+unsigned long long t_bound(unsigned long long a, unsigned long long w, unsigned long long i)
+{ return ltx::work_bound(a, w, i); }
+unsigned long long t_owner(unsigned long long a, unsigned long long w, unsigned long long x)
+{ return ltx::work_owner(a, w, x); }
 int t_clamp(int v, int lo, int hi) { return ltx::clamp_int(v, lo, hi); }
 }
 """
@@ -75,3 +85,53 @@ def test_key_ranges(idx):
 def test_clamp(idx):
     for v in (-2 ** 31, -1, 0, 5, 7, 2 ** 31 - 1):
         assert 0 <= idx.t_clamp(v, 0, 7) <= 7
+
+
+def test_pages_of_a_run_of_tokens(idx):
+    """Every token of a run lies on one of the pages that its work slots cover, and
+    what leaves the table, or names no page, is told apart."""
+    import ctypes
+    out = (ctypes.c_int * 3)()
+    rng = random.Random(2)
+    for _ in range(400):
+        start, n = rng.randint(0, 300), rng.choice([1, 2, 63, 64, 65, 66, rng.randint(1, 500)])
+        tokens = []
+        for i in range(1 if n == 1 else -(-n // 64) + 1):
+            idx.t_span(start, n, i, out)
+            block, a, b = out
+            if b > a:
+                assert a // 64 == (b - 1) // 64 == block
+                tokens += range(a, b)
+        assert tokens == list(range(start, start + n))
+        idx.t_span(start, n, -(-n // 64) + 1, out)     # past the last
+        assert out[2] <= out[1]
+    big = 2 ** 31 - 1
+    assert idx.t_span_ok(0, 64, 64) and idx.t_span_ok(64, 0, 64) and idx.t_span_ok(10, 54, 64)
+    for start, n, cap in ((-1, 1, 64), (-2 ** 31, 1, 64), (64, 1, 64), (10, 55, 64), (65, 0, 64),
+                          (big, 1, 64), (big, big, 64), (1, big, 64)):
+        assert not idx.t_span_ok(start, n, cap), (start, n, cap)
+    assert idx.t_page_ok(0, 3) and idx.t_page_ok(2, 3)
+    for page, pages in ((-1, 3), (3, 3), (0, 0), (big, 3), (-2 ** 31, 3)):
+        assert not idx.t_page_ok(page, pages)
+
+
+def test_equal_runs_of_work(idx):
+    """Runs cover the list in order, each of at least one item and of sizes that
+    differ by one; the owner of an item is the run it lies in."""
+    import ctypes
+    u = ctypes.c_ulonglong
+    idx.t_bound.restype = idx.t_owner.restype = u
+    rng = random.Random(3)
+    for _ in range(200):
+        all_ = rng.choice([1, 2, 7, rng.randint(1, 5000)])
+        workers = min(all_, rng.choice([1, 2, 1184, rng.randint(1, 1184)]))
+        b = [idx.t_bound(u(all_), u(workers), u(i)) for i in range(workers + 1)]
+        assert b[0] == 0 and b[-1] == all_
+        sizes = {y - x for x, y in zip(b, b[1:])}
+        assert min(sizes) >= 1 and max(sizes) - min(sizes) <= 1
+        for i in range(workers):
+            for x in {b[i], b[i + 1] - 1}:
+                assert idx.t_owner(u(all_), u(workers), u(x)) == i
+    big = 1 << 40                                       # beyond 32 bits
+    assert idx.t_owner(u(big), u(1184), u(big - 1)) == 1183
+    assert idx.t_bound(u(big), u(1184), u(1184)) == big

@@ -41,6 +41,7 @@
 #include "block_ops.h"
 #include "kernels.h"
 #include "packed_index.h"
+#include "packed_seq.cuh"
 #include "ptx.cuh"
 
 namespace ltx {
@@ -120,24 +121,6 @@ __device__ __forceinline__ void tma_load_3d(const void* map, uint64_t* bar, void
       "tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
-}
-
-// The sequence that owns work slot `slot`: the last s with slot_base <= slot.
-// The whole warp searches, 32 ways at a time.
-__device__ __forceinline__ int find_seq(const int* cu, int seqs, int rows, int tile, int extra,
-                                        int slot)
-{
-  int lo = 0, hi = seqs;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int at = lo + (int)lane_id() * step;
-    const bool below = lane_id() == 0 ||
-        (at < hi && slot_base(clamp_int(cu[at], 0, rows), at, tile, extra) <= slot);
-    const int last = 31 - __clz((int)__ballot_sync(0xffffffffu, below));
-    lo += last * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
 }
 
 // Columns [col0, col0 + D / 2) of one output row from the keys [lo, hi) of its

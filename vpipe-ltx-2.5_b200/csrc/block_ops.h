@@ -143,4 +143,34 @@ struct PackedAttention {
 };
 int launch_attention_packed(const PackedAttention& a, int* err, cudaStream_t s);
 
+// The 8-bit key/value cache (kv8.cu).  Codes int8 [pages][kv_heads][64][D],
+// bf16 scales [pages][kv_heads]; head_dim 64, 128 or 256.
+struct Kv8Cache {
+  int8_t *k = nullptr, *v = nullptr;
+  uint16_t *ks = nullptr, *vs = nullptr;
+  int pages = 0, kv_heads = 0, head_dim = 0;
+};
+// Packed rows and the pages of their sequences: rows [cu[s], cu[s + 1]) of
+// sequence s at the tokens from starts[s] on (attention: the last ones of
+// starts[s] tokens); table [seqs][table_ld].  All device int32.
+struct Kv8Rows {
+  const int *cu = nullptr, *starts = nullptr, *table = nullptr;
+  int table_ld = 0, seqs = 0, rows = 0;
+};
+int launch_kv8_append(const Kv8Cache& c, const Kv8Rows& r, const __nv_bfloat16* k, int ldk,
+                      const __nv_bfloat16* v, int ldv, int* err, cudaStream_t s);
+int launch_kv8_read(const Kv8Cache& c, const Kv8Rows& r, __nv_bfloat16* k, int ldk,
+                    __nv_bfloat16* v, int ldv, int* err, cudaStream_t s);
+struct Kv8Attention {
+  Kv8Cache cache;
+  Kv8Rows rows;
+  const __nv_bfloat16* q = nullptr;
+  __nv_bfloat16* o = nullptr;
+  int ldq = 0, ldo = 0, heads = 0, max_len = 0, window = 0;
+  float scale = 0.0f;
+  float* workspace = nullptr;
+};
+size_t kv8_attention_workspace(int head_dim, int num_sms);
+int launch_kv8_attention(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s);
+
 }  // namespace ltx

@@ -44,4 +44,37 @@ LTX_HD int key_low(int pos, int window)
   return window > 0 && pos >= window ? pos - window + 1 : 0;
 }
 
+// ---- the paged cache -------------------------------------------------------
+
+constexpr int kPage = 64;         // tokens of a page
+
+// Whether n tokens from `start` on lie inside a table of `cap` tokens.
+LTX_HD bool span_ok(int start, int n, int cap)
+{
+  return start >= 0 && start <= cap && n <= cap - start;
+}
+LTX_HD bool page_ok(int page, int pages) { return page >= 0 && page < pages; }
+
+// The tokens [a, b) of [start, start + n) on the i-th page they touch, page
+// `block` of the sequence; b <= a where there is no i-th page.
+struct PageSpan {
+  int block, a, b;
+};
+LTX_HD PageSpan page_span(int start, int n, int i)
+{
+  PageSpan r;
+  r.block = start / kPage + i;
+  const int from = r.block * kPage;
+  r.a = start > from ? start : from;
+  r.b = start + n < from + kPage ? start + n : from + kPage;
+  return r;
+}
+
+// A list of `all` work items in equal runs: worker i of `workers` (at most
+// `all`) has the items [work_bound(i), work_bound(i + 1)); item x is
+// work_owner's.
+typedef unsigned long long u64;
+LTX_HD u64 work_bound(u64 all, u64 workers, u64 i) { return all * i / workers; }
+LTX_HD u64 work_owner(u64 all, u64 workers, u64 x) { return ((x + 1) * workers - 1) / all; }
+
 }  // namespace ltx

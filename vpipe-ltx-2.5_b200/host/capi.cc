@@ -730,6 +730,124 @@ int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const void* k, in
   });
 }
 
+namespace {
+
+ltx::Kv8Cache to_cache(const ltx_kv8_cache* c)
+{
+  ltx::Kv8Cache o;
+  o.k = c->k;
+  o.v = c->v;
+  o.ks = c->k_scale;
+  o.vs = c->v_scale;
+  o.pages = c->pages;
+  o.kv_heads = c->kv_heads;
+  o.head_dim = c->head_dim;
+  return o;
+}
+
+ltx::Kv8Rows to_rows(const int32_t* cu, const int32_t* starts, const int32_t* table, int table_ld,
+                     int seqs, int rows)
+{
+  ltx::Kv8Rows r;
+  r.cu = cu;
+  r.starts = starts;
+  r.table = table;
+  r.table_ld = table_ld;
+  r.seqs = seqs;
+  r.rows = rows;
+  return r;
+}
+
+}  // namespace
+
+int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,
+                   const void* v, int ldv, const int32_t* cu, const int32_t* starts,
+                   const int32_t* table, int table_ld, int seqs, int rows, void* stream)
+{
+  return guarded([&]() -> int {
+    OnDevice on_(dev_of(ctx));
+    if (ctx == nullptr) return LTX_E_NULL;
+    if (cache == nullptr) return fail(ctx, LTX_E_NULL, "kv8_append: cache is null");
+    const ltx::Kv8Cache c = to_cache(cache);
+    const ltx::Kv8Rows r = to_rows(cu, starts, table, table_ld, seqs, rows);
+    std::string e;
+    const int rc = ltx25::check_kv8_rows("kv8_append", c, r, k, ldk, v, ldv, &e);
+    if (rc != LTX_OK) return fail(ctx, rc, e);
+    if (seqs == 0 || rows == 0) return LTX_OK;
+    if (ltx::launch_kv8_append(c, r, static_cast<const __nv_bfloat16*>(k), ldk,
+                               static_cast<const __nv_bfloat16*>(v), ldv, ctx->ops.err_word(),
+                               S(stream)) != 0)
+      return fail(ctx, LTX_E_CUDA, "kv8_append launch failed");
+    return LTX_OK;
+  });
+}
+
+int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int ldk, void* v, int ldv,
+                 const int32_t* cu, const int32_t* starts, const int32_t* table, int table_ld,
+                 int seqs, int rows, void* stream)
+{
+  return guarded([&]() -> int {
+    OnDevice on_(dev_of(ctx));
+    if (ctx == nullptr) return LTX_E_NULL;
+    if (cache == nullptr) return fail(ctx, LTX_E_NULL, "kv8_read: cache is null");
+    const ltx::Kv8Cache c = to_cache(cache);
+    const ltx::Kv8Rows r = to_rows(cu, starts, table, table_ld, seqs, rows);
+    std::string e;
+    const int rc = ltx25::check_kv8_rows("kv8_read", c, r, k, ldk, v, ldv, &e);
+    if (rc != LTX_OK) return fail(ctx, rc, e);
+    if (seqs == 0 || rows == 0) return LTX_OK;
+    if (ltx::launch_kv8_read(c, r, static_cast<__nv_bfloat16*>(k), ldk,
+                             static_cast<__nv_bfloat16*>(v), ldv, ctx->ops.err_word(),
+                             S(stream)) != 0)
+      return fail(ctx, LTX_E_CUDA, "kv8_read launch failed");
+    return LTX_OK;
+  });
+}
+
+int ltx_kv8_attention_workspace(ltx_ctx* ctx, int head_dim, size_t* bytes)
+{
+  return guarded([&]() -> int {
+    if (ctx == nullptr) return LTX_E_NULL;
+    if (bytes == nullptr) return fail(ctx, LTX_E_NULL, "kv8_attention_workspace: null");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+      return fail(ctx, LTX_E_SHAPE, "kv8_attention_workspace: need head_dim 64, 128 or 256");
+    *bytes = ltx::kv8_attention_workspace(head_dim, ctx->ops.num_sms());
+    return LTX_OK;
+  });
+}
+
+int ltx_kv8_attention(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* q, int ldq, void* o,
+                      int ldo, const int32_t* cu_q, const int32_t* lengths, const int32_t* table,
+                      int table_ld, int seqs, int rows, int heads, int max_len, int window,
+                      float scale, void* workspace, size_t workspace_bytes, void* stream)
+{
+  return guarded([&]() -> int {
+    OnDevice on_(dev_of(ctx));
+    if (ctx == nullptr) return LTX_E_NULL;
+    if (cache == nullptr) return fail(ctx, LTX_E_NULL, "kv8_attention: cache is null");
+    ltx::Kv8Attention a;
+    a.cache = to_cache(cache);
+    a.rows = to_rows(cu_q, lengths, table, table_ld, seqs, rows);
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.o = static_cast<__nv_bfloat16*>(o);
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.heads = heads;
+    a.max_len = max_len;
+    a.window = window;
+    a.scale = scale;
+    a.workspace = static_cast<float*>(workspace);
+    const size_t need = ltx::kv8_attention_workspace(a.cache.head_dim, ctx->ops.num_sms());
+    std::string e;
+    const int rc = ltx25::check_kv8_attention(a, workspace_bytes, need, &e);
+    if (rc != LTX_OK) return fail(ctx, rc, e);
+    if (seqs == 0 || rows == 0) return LTX_OK;
+    if (ltx::launch_kv8_attention(a, ctx->ops.num_sms(), ctx->ops.err_word(), S(stream)) != 0)
+      return fail(ctx, LTX_E_CUDA, "kv8_attention launch failed");
+    return LTX_OK;
+  });
+}
+
 }  // extern "C"
 
 struct ltx_block {

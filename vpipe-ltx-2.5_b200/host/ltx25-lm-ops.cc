@@ -1,6 +1,7 @@
 // ltx25-lm-ops.cc -- argument checks of the language-model operators.
 #include "ltx25-lm-ops.h"
 
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -71,7 +72,76 @@ int check_ints(const char* op, const char* name, const int* p, std::string* why)
   return LTX_OK;
 }
 
+// the cache's buffers, and the offsets, starts and table of its sequences
+int check_cache(const char* op, const ltx::Kv8Cache& c, const ltx::Kv8Rows& r, std::string* why)
+{
+  const std::string o(op);
+  if (c.kv_heads <= 0 || c.kv_heads > 65535 || c.pages < 0 ||
+      (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)) {
+    *why = o + ": need pages >= 0, kv_heads 1..65535, head_dim 64, 128 or 256";
+    return LTX_E_SHAPE;
+  }
+  if (r.seqs < 0 || r.rows < 0 || r.seqs > (1 << 29) || r.table_ld < 1 || r.table_ld > (1 << 24)) {
+    *why = o + ": need seqs 0..2^29, rows >= 0, table columns 1..2^24";
+    return LTX_E_SHAPE;
+  }
+  if (r.seqs == 0 || r.rows == 0) return LTX_OK;
+  if (c.k == nullptr || c.v == nullptr || c.ks == nullptr || c.vs == nullptr) {
+    *why = o + ": a cache buffer is null";
+    return LTX_E_NULL;
+  }
+  if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.ks, 2) || !aligned(c.vs, 2)) {
+    *why = o + ": cache codes must be 16-byte, scales 2-byte aligned";
+    return LTX_E_ALIGN;
+  }
+  int rc;
+  if ((rc = check_ints(op, "cu", r.cu, why)) != LTX_OK ||
+      (rc = check_ints(op, "starts / lengths", r.starts, why)) != LTX_OK)
+    return rc;
+  return check_ints(op, "table", r.table, why);
+}
+
 }  // namespace
+
+int check_kv8_rows(const char* op, const ltx::Kv8Cache& c, const ltx::Kv8Rows& r, const void* k,
+                   int ldk, const void* v, int ldv, std::string* why)
+{
+  int rc = check_cache(op, c, r, why);
+  if (rc != LTX_OK || r.seqs == 0) return rc;
+  const long long cols = (long long)c.kv_heads * c.head_dim;
+  if ((rc = check_rows(op, "k", k, ldk, r.rows, cols, why)) != LTX_OK) return rc;
+  return check_rows(op, "v", v, ldv, r.rows, cols, why);
+}
+
+int check_kv8_attention(const ltx::Kv8Attention& a, size_t workspace_bytes, size_t need,
+                        std::string* why)
+{
+  const char* op = "kv8_attention";
+  int rc = check_heads(op, a.heads, a.cache.kv_heads, a.cache.head_dim, a.window, a.scale, why);
+  if (rc != LTX_OK || (rc = check_cache(op, a.cache, a.rows, why)) != LTX_OK) return rc;
+  if ((long long)a.rows.rows * a.heads > INT_MAX || a.max_len < 0) {
+    *why = "kv8_attention: need rows * heads < 2^31 and max_len >= 0";
+    return LTX_E_SHAPE;
+  }
+  if (a.rows.seqs == 0 || a.rows.rows == 0) return LTX_OK;
+  const long long cols = (long long)a.heads * a.cache.head_dim;
+  if ((rc = check_rows(op, "q", a.q, a.ldq, a.rows.rows, cols, why)) != LTX_OK ||
+      (rc = check_rows(op, "o", a.o, a.ldo, a.rows.rows, cols, why)) != LTX_OK)
+    return rc;
+  if (a.workspace == nullptr) {
+    *why = "kv8_attention: workspace is null";
+    return LTX_E_NULL;
+  }
+  if (!aligned(a.workspace, 16)) {
+    *why = "kv8_attention: workspace must be 16-byte aligned";
+    return LTX_E_ALIGN;
+  }
+  if (workspace_bytes < need) {
+    *why = "kv8_attention: need a workspace of " + std::to_string(need) + " bytes";
+    return LTX_E_SHAPE;
+  }
+  return LTX_OK;
+}
 
 int check_attention_packed(const ltx::PackedAttention& a, std::string* why)
 {

@@ -106,6 +106,11 @@ SIGNATURES = {
                            _I, _I, _P]),
     "ltx_attention_packed": (_I, [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P, _P] + [_I] * 8
                              + [ctypes.c_float, _P]),
+    "ltx_kv8_append": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _P]),
+    "ltx_kv8_read": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _P]),
+    "ltx_kv8_attention_workspace": (_I, [_P, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "ltx_kv8_attention": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _P] + [_I] * 6
+                          + [ctypes.c_float, _P, ctypes.c_size_t, _P]),
     "ltx_block_create": (_I, [_P, _I, _I, _I, _I, ctypes.POINTER(_P)]),
     "ltx_block_destroy": (None, [_P]),
     "ltx_block_last_error": (ctypes.c_char_p, [_P]),
@@ -825,6 +830,135 @@ def attention_packed(ctx, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal
         k.shape[0], heads, kv_heads, head_dim, int(causal), window,
         head_dim ** -0.5 if scale is None else scale, _stream_of(ctx, stream)),
         "attention_packed")
+    return out
+
+
+class _KV8Struct(ctypes.Structure):
+    """ltx_kv8_cache (include/ltx25_cuda.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("pages", _I),
+                ("kv_heads", _I), ("head_dim", _I)]
+
+
+class KV8Cache:
+    """An 8-bit key/value cache over the caller's device tensors: int8 codes k and v
+    [pages][kv_heads][64][head_dim] and bf16 scales [pages][kv_heads] (see
+    ltx_kv8_cache).  `KV8Cache.empty` allocates one."""
+
+    PAGE = 64
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        _need(k.dim() == 4 and k.shape[2] == self.PAGE and k.shape == v.shape, -2,
+              f"KV8Cache: need codes [pages][kv_heads][64][head_dim], got {tuple(k.shape)} and "
+              f"{tuple(v.shape)}")
+        self.pages, self.kv_heads, _, self.head_dim = k.shape
+        for t, dt, shape in ((k, torch.int8, k.shape), (v, torch.int8, k.shape),
+                             (k_scale, torch.bfloat16, k.shape[:2]),
+                             (v_scale, torch.bfloat16, k.shape[:2])):
+            _need(t.dtype == dt and t.shape == shape and t.is_contiguous() and
+                  t.device == k.device, -2,
+                  f"KV8Cache: need a contiguous {dt} tensor {tuple(shape)} on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._c = _KV8Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                             self.pages, self.kv_heads, self.head_dim)
+
+    @classmethod
+    def empty(cls, ctx, pages, kv_heads, head_dim):
+        import torch
+        dev = torch.device("cuda", ctx.device)
+        codes = (pages, kv_heads, cls.PAGE, head_dim)
+        return cls(torch.empty(codes, dtype=torch.int8, device=dev),
+                   torch.empty(codes, dtype=torch.int8, device=dev),
+                   torch.empty(codes[:2], dtype=torch.bfloat16, device=dev),
+                   torch.empty(codes[:2], dtype=torch.bfloat16, device=dev))
+
+    def _on(self, ctx):
+        d = self.k.device
+        _need(d.type == "cuda" and d.index == ctx.device, -2,
+              f"KV8Cache: need a cache on cuda:{ctx.device}, got {d}")
+        return ctypes.byref(self._c)
+
+
+def _table(ctx, table, seqs):
+    import torch
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == seqs and
+          table.is_contiguous(), -2,
+          f"table: need contiguous int32 [{seqs}][columns], got {tuple(table.shape)} {table.dtype}")
+    _need(table.device.type == "cuda" and table.device.index == ctx.device, -2,
+          f"table: need a tensor on cuda:{ctx.device}, got {table.device}")
+    return _ptr(table), table.shape[1]
+
+
+def kv8_append(ctx, cache, k, v, cu, starts, table, stream=None):
+    """ltx_kv8_append: rows cu[s] + i of k and v [rows][kv_heads * head_dim] (bf16)
+    become tokens starts[s] + i of sequence s.  cu int32 [seqs + 1], starts int32
+    [seqs], table int32 [seqs][columns], all on the device."""
+    seqs, cols = cu.numel() - 1, cache.kv_heads * cache.head_dim
+    ldk, ldv = _rows(ctx, k, cols, "k"), _rows(ctx, v, cols, "v")
+    _need(k.shape[0] == v.shape[0], -2, "kv8_append: k and v differ in rows")
+    pt, tld = _table(ctx, table, seqs)
+    ctx._ok(ctx.lib.ltx_kv8_append(
+        ctx.h, cache._on(ctx), _ptr(k), ldk, _ptr(v), ldv, _ints(ctx, cu, seqs + 1, "cu"),
+        _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, k.shape[0], _stream_of(ctx, stream)),
+        "kv8_append")
+
+
+def kv8_read(ctx, cache, cu, starts, table, rows, k=None, v=None, stream=None):
+    """ltx_kv8_read: tokens starts[s] + i of the sequences back as bf16 rows
+    cu[s] + i of k and v [rows][kv_heads * head_dim] (new tensors by default);
+    returns (k, v)."""
+    import torch
+    seqs, cols = cu.numel() - 1, cache.kv_heads * cache.head_dim
+    make = lambda: torch.empty((rows, cols), dtype=torch.bfloat16,             # noqa: E731
+                               device=cache.k.device)
+    k = _new_on(ctx, stream, make) if k is None else k
+    v = _new_on(ctx, stream, make) if v is None else v
+    ldk, ldv = _rows(ctx, k, cols, "k"), _rows(ctx, v, cols, "v")
+    _need(k.shape[0] == rows and v.shape[0] == rows, -2, "kv8_read: k and v need `rows` rows")
+    pt, tld = _table(ctx, table, seqs)
+    ctx._ok(ctx.lib.ltx_kv8_read(
+        ctx.h, cache._on(ctx), _ptr(k), ldk, _ptr(v), ldv, _ints(ctx, cu, seqs + 1, "cu"),
+        _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, rows, _stream_of(ctx, stream)),
+        "kv8_read")
+    return k, v
+
+
+def kv8_attention_workspace(ctx, head_dim):
+    """Bytes of kv8_attention's workspace, whatever the lengths."""
+    n = ctypes.c_size_t(0)
+    ctx._ok(ctx.lib.ltx_kv8_attention_workspace(ctx.h, head_dim, ctypes.byref(n)),
+            "kv8_attention_workspace")
+    return n.value
+
+
+def kv8_attention(ctx, cache, q, cu_q, lengths, table, heads, max_len, window=0, scale=None,
+                  out=None, workspace=None, stream=None):
+    """ltx_kv8_attention: the rows of q [rows][heads * head_dim] (bf16), the last
+    tokens of sequences whose lengths[s] tokens the cache holds, over those tokens.
+    scale: 1/sqrt(head_dim) by default; workspace: a device tensor of
+    kv8_attention_workspace bytes (a new one by default; calls that may overlap
+    need one each).  Returns [rows][heads * head_dim]."""
+    import torch
+    seqs, D = cu_q.numel() - 1, cache.head_dim
+    rows = q.shape[0]
+    ldq = _rows(ctx, q, heads * D, "q")
+    if out is None:
+        out = _new_on(ctx, stream, lambda: torch.empty((rows, heads * D), dtype=q.dtype,
+                                                       device=q.device))
+    ldo = _rows(ctx, out, heads * D, "out")
+    _need(out.shape[0] == rows, -2, "kv8_attention: out and q differ in rows")
+    pt, tld = _table(ctx, table, seqs)
+    if workspace is None:
+        need = kv8_attention_workspace(ctx, D)
+        workspace = _new_on(ctx, stream, lambda: torch.empty(need, dtype=torch.uint8,
+                                                             device=q.device))
+    _need(workspace.device == q.device and workspace.is_contiguous(), -2,
+          f"workspace: need a contiguous tensor on {q.device}")
+    ctx._ok(ctx.lib.ltx_kv8_attention(
+        ctx.h, cache._on(ctx), _ptr(q), ldq, _ptr(out), ldo, _ints(ctx, cu_q, seqs + 1, "cu_q"),
+        _ints(ctx, lengths, seqs, "lengths"), pt, tld, seqs, rows, heads, max_len, window,
+        D ** -0.5 if scale is None else scale, _ptr(workspace),
+        workspace.numel() * workspace.element_size(), _stream_of(ctx, stream)), "kv8_attention")
     return out
 
 
