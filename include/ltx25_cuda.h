@@ -365,7 +365,7 @@ LTX_API int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const voi
 /* An 8-bit key/value cache: pages of LTX_KV8_PAGE tokens in the caller's
  * device memory.  Codes are int8 [pages][kv_heads][LTX_KV8_PAGE][head_dim],
  * with one bf16 scale for each page and head ([pages][kv_heads]), keys and
- * values each; a code c stands for c * scale.  Token t of sequence s is slot
+ * values each, not negative; a code c stands for c * scale.  Token t of sequence s is slot
  * t % LTX_KV8_PAGE of page table[s][t / LTX_KV8_PAGE] (table_ld columns).  A
  * page's content needs no clearing before its first use.  Sequences may share
  * pages that nothing is appended to.
@@ -412,9 +412,9 @@ LTX_API int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int 
  * token a sequence is the usual call; the cache is read once for each 16 rows
  * (tokens times the query heads of a key/value head).  max_len sizes the
  * launch: the largest length expected.  The workspace is the caller's,
- * ltx_kv8_attention_workspace bytes whatever the lengths, 16-byte aligned; two
- * calls that may run at once (streams, captured graphs) need one each.
- * Allocates nothing. */
+ * ltx_kv8_attention_workspace bytes whatever the lengths, 16-byte aligned, of
+ * any content; two calls that may run at once (streams, captured graphs) need
+ * one each.  Allocates nothing. */
 LTX_API int ltx_kv8_attention_workspace(ltx_ctx* ctx, int head_dim, size_t* bytes);
 LTX_API int ltx_kv8_attention(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* q, int ldq,
                               void* o, int ldo, const int32_t* cu_q, const int32_t* lengths,

@@ -286,9 +286,10 @@ def test_rows_behind_the_last_sequence_and_given_workspaces(ctx):
     assert torch.all(out[:2] == 7.0) and torch.all(out[6:] == 7.0)
 
 
-def test_two_streams_and_two_graphs(ctx):
-    """Calls that run at once, each with its own workspace, and graphs replayed after
-    lengths and pages changed on the device."""
+@pytest.mark.parametrize("given", [True, False])
+def test_two_streams_and_two_graphs(ctx, given):
+    """Calls that run at once, each with a workspace of its own (given, or left to the
+    call), and graphs replayed after lengths changed on the device."""
     import torch
     import ltx25_b200 as L
     heads, kv_heads, D, S = 8, 2, 128, 6
@@ -300,7 +301,8 @@ def test_two_streams_and_two_graphs(ctx):
     state = []
     for i, st in enumerate(streams):
         q, ln = rows_of(S, heads * D, i), ints([1] * S)
-        ws = torch.empty(L.kv8_attention_workspace(ctx, D), device="cuda", dtype=torch.uint8)
+        ws = torch.empty(L.kv8_attention_workspace(ctx, D), device="cuda",
+                         dtype=torch.uint8) if given else None
         out = torch.empty_like(q)
         torch.cuda.synchronize()
         run = lambda q=q, ln=ln, ws=ws, out=out: L.kv8_attention(          # noqa: E731

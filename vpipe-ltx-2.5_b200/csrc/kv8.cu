@@ -13,6 +13,8 @@
 #include <climits>
 #include <cstring>
 
+#include <cuda_fp16.h>
+
 #include "attention_tc.cuh"
 #include "block_ops.h"
 #include "kernels.h"
@@ -216,39 +218,54 @@ __global__ void __launch_bounds__(kAppendThreads)
 // ---- attention over the cache ----------------------------------------------
 //
 // The new rows of a sequence (n tokens, the last n of its `length`) times the
-// G query heads of a key/value head are rows token * G + head, in tiles of 16:
-// one warp MMA's rows.  The work is the list of all (sequence, kv head, row
-// tile, 8 KB stage of keys and values) in that order, and every warp of the
-// grid takes an equal run of it, whatever the lengths: at most its first and
-// its last tile are shared with other warps.  A tile that one warp has whole
-// goes straight to o; the others leave (max, sum, O) in the workspace for
-// kv8_merge_kernel.
+// G query heads of a key/value head are rows token * G + head, in tiles of 8
+// or 16.  The work is the list of all (sequence, kv head, row tile, 8 KB stage
+// of keys and values) in that order, and every warp of the grid takes an equal
+// run of it, whatever the lengths, and works on it alone: no barrier, no shared
+// result.  A tile that one warp has whole goes straight to o; of the others
+// (a warp's first and last, at most) each part goes to the workspace as (max,
+// sum, O) for kv8_merge_kernel.  Measured beside this on 64 ragged sequences
+// and on 32 of one-row tiles (8192 and 4096 tokens at most): runs shared by a
+// block's four warps with a join in shared memory, and parts joined by the last
+// block to arrive, which saves the second launch: 104 and 53 us, half of it
+// waiting at barriers, fences and counters in the middle of a run.
 //
 // This reads 2 D bytes a token and key head and is bound by HBM as long as a
-// code costs few instructions: int8 -> f16 is a byte permute into 1024 + u and
-// one packed subtraction (exact), the products run on warp MMAs with f32 sums
-// (m16n8k16), K's scale goes into the exponent's factor and V's into P.  Codes
-// and P are f16 (P rounds at 2^-11); q, whose 8 bits f16 holds exactly, is
-// brought near 2^8 by a power of two a row.
+// code costs few instructions.  The products run transposed, S^T = K Q^T and
+// O^T = V^T P^T, on warp MMAs with f32 sums (m16n8k16, f16 operands): 16 keys or
+// 16 output columns by 8 query rows, since a decoded token has no more rows than
+// query heads share a key head.  Against 16 query rows in the M place that halves
+// the MMAs, the exponentials and the registers (measured on 131072 tokens, 8 key
+// heads of 128: 895 to 4xx instructions a stage and warp).  P rounds at 2^-11; q's
+// 8 bits are exact once its row is brought near 2^8 by a power of two.
+//   K  byte 128 + c in the low half of an f16 is the subnormal (128 + c) 2^-24:
+//      one byte permute a pair, and 128 sum(q) leaves the score with the
+//      exponent's other constants.
+//   V  the pair becomes 1024 + 128 + c by a permute, and c by one packed
+//      subtraction (exact): here 128 sum(P) would swamp the f32 sums.
+//   P  leaves S^T's accumulators key by lane group and enters the second product
+//      row by lane group: one 8x8 transposition a 16-bit register.
+// K's scale goes into the exponent's factor, V's as a power of two into P's
+// exponent, so neither costs an instruction a score.
 //
-// Each warp streams its stages through a ring of its own with 16-byte
-// asynchronous copies (no barrier between warps).  Shared memory is swizzled
-// by 16-byte pieces so that the fragment reads below are free of conflicts:
-// keys of one MMA column group for K, pairs of keys for V.
+// Each warp streams its stages through a ring of its own, keys and values in
+// turn, two stages ahead, with 16-byte asynchronous copies (no barrier between
+// warps before a tile ends).  Shared memory is swizzled by 16-byte pieces so
+// that the fragment reads below are free of conflicts: eight keys for K, pairs
+// of keys for V.
 
-template <int D>
+template <int D, int NR>
 struct KvCfg {
   static constexpr int kTok = 4096 / D;                // tokens of a stage
-  static constexpr int kStages = 3;
-  static constexpr int kWarps = 4;
+  // warps of the block that has an SM to itself: as many as the registers allow
+  static constexpr int kWarps = D == 256 || NR == 2 ? 8 : 12;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kStageBytes = 8192;             // K, then V
-  static constexpr int kWarpBytes = kStages * kStageBytes + kStages * 16;
-  static constexpr int kSmem = kWarps * kWarpBytes;
-  static constexpr int kNT = kTok / 8;                 // score column tiles
-  static constexpr int kOT = D / 8;                    // output column tiles
+  static constexpr int kSmem = kWarps * 2 * kStageBytes;
+  static constexpr int kMT = kTok / 16;                // key tiles of a stage
+  static constexpr int kOT = D / 16;                   // output column tiles
 };
 
-constexpr int kTileRows = 16;
 constexpr float kKvGrow = 6.0f;   // log2 of the largest P before O is rescaled
 
 struct KvAttn {
@@ -261,8 +278,8 @@ struct KvAttn {
   int table_ld, pages, kv_heads, group, seqs, rows, window;
   float c;                        // scale log2 e
   int workers;                    // warps of the attention grid
-  float* part_o;                  // [workers][2][16][D]
-  float* part_ml;                 // [workers][2][16][2]
+  float* part_o;                  // [workers][2][tile rows][D]
+  float* part_ml;                 // [workers][2][tile rows][2]
   int* err;
 };
 
@@ -272,111 +289,133 @@ struct KvSeq {
   int tiles, first, units;        // row tiles; first stage and stages of each
 };
 
-template <int D>
+template <int D, int TR>
 __device__ __forceinline__ KvSeq kv_seq(const KvAttn& p, int s)
 {
-  constexpr int T = KvCfg<D>::kTok;
+  constexpr int T = 4096 / D;                          // tokens of a stage
   KvSeq q;
   q.row0 = clamp_int(p.cu[s], 0, p.rows);
   q.n = clamp_int(p.cu[s + 1], q.row0, p.rows) - q.row0;
   const int len = p.lengths[s], cap = p.table_ld * kPage;
   q.len = clamp_int(len, 0, cap);
   if (len != q.len) atomicCAS(p.err, 0, KERR_PLACE);
-  q.tiles = (q.n * p.group + kTileRows - 1) / kTileRows;
+  q.tiles = (q.n * p.group + TR - 1) / TR;
   const int lo = key_low(q.len - q.n, p.window);
   q.first = lo / T;
   q.units = q.len > lo ? (q.len + T - 1) / T - q.first : 0;
   return q;
 }
 
-template <int D>
 __device__ __forceinline__ u64 kv_work(const KvAttn& p, const KvSeq& q)
 {
   return (u64)q.tiles * (u64)p.kv_heads * (u64)q.units;
 }
 
-// pre[t] = work of the sequences before thread t's (an equal run of them each);
-// pre[N] = all of it.  Every thread of the block calls it.
-template <int D, int N>
-__device__ __forceinline__ void kv_plan(const KvAttn& p, u64* pre)
+// Warps that share `all` stages: one at least for each.
+__device__ __forceinline__ u64 kv_workers(const KvAttn& p, u64 all)
 {
-  __shared__ u64 s_warp[N / 32];
+  return min((u64)p.workers, all);
+}
+
+// All sequences of a call as the first N threads of a block see them: the work
+// before each thread's run of them (`each` from threadIdx * each on) and, where a
+// thread has one at most, what they ask for.
+template <int N>
+struct KvTable {
+  u64 before[N + 1];
+  u64 warp_sum[N / 32];
+  KvSeq q[N];
+};
+
+// Fills it; every thread of the block calls this.
+template <int D, int TR, int N>
+__device__ __forceinline__ void kv_scan(const KvAttn& p, KvTable<N>& tab)
+{
   const int each = (p.seqs + N - 1) / N;
   const int t = (int)threadIdx.x, lane = t & 31;
   u64 mine = 0;
-  for (int s = t * each; s < min(p.seqs, (t + 1) * each); ++s)
-    mine += kv_work<D>(p, kv_seq<D>(p, s));
+  for (int i = 0; t < N && i < each; ++i) {
+    const int s = t * each + i;
+    if (s >= p.seqs) break;
+    const KvSeq q = kv_seq<D, TR>(p, s);
+    if (each == 1) tab.q[t] = q;
+    mine += kv_work(p, q);
+  }
   u64 sum = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const u64 o = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += o;
   }
-  if (lane == 31) s_warp[t >> 5] = sum;
+  if (lane == 31 && t < N) tab.warp_sum[t >> 5] = sum;
   __syncthreads();
-  u64 before = 0;
+  u64 earlier = 0;
 #pragma unroll
   for (int w = 0; w < N / 32; ++w)
-    if (w < (t >> 5)) before += s_warp[w];
-  pre[t + 1] = before + sum;
-  if (t == 0) pre[0] = 0;
+    if (w < (t >> 5)) earlier += tab.warp_sum[w];
+  if (t < N) tab.before[t] = earlier + sum - mine;
+  if (t == N - 1) tab.before[N] = earlier + sum;
   __syncthreads();
 }
 
-// The sequence that work item x falls into, and the work before it.
-template <int D, int N>
-__device__ __forceinline__ int kv_find(const KvAttn& p, const u64* pre, u64 x, u64* before)
+template <int D, int TR, int N>
+__device__ __forceinline__ KvSeq kv_get(const KvAttn& p, const KvTable<N>& tab, int s)
+{
+  return p.seqs <= N ? tab.q[s] : kv_seq<D, TR>(p, s);
+}
+
+// A place in the list of work.
+struct KvPlace {
+  KvSeq q;
+  int s, head, tile, unit;
+};
+
+// The place of stage x.
+template <int D, int TR, int N>
+__device__ __forceinline__ KvPlace kv_locate(const KvAttn& p, const KvTable<N>& tab, u64 x)
 {
   int lo = 0, hi = N;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (pre[mid] <= x) lo = mid;
+    if (tab.before[mid] <= x) lo = mid;
     else hi = mid;
   }
   const int each = (p.seqs + N - 1) / N;
-  int s = lo * each;
-  u64 at = pre[lo];
-  const int last = min(p.seqs, (lo + 1) * each) - 1;
-  while (s < last) {
-    const u64 w = kv_work<D>(p, kv_seq<D>(p, s));
-    if (x < at + w) break;
+  KvPlace a;
+  u64 at = tab.before[lo];
+  a.s = lo * each;
+  const int last = min(p.seqs, a.s + each) - 1;
+  while (true) {
+    a.q = kv_get<D, TR, N>(p, tab, a.s);
+    const u64 w = kv_work(p, a.q);
+    if (x < at + w || a.s == last) break;
     at += w;
-    ++s;
+    ++a.s;
   }
-  *before = at;
-  return s;
+  const u64 per = (u64)a.q.tiles * (u64)a.q.units, in = x - at;
+  a.head = (int)(in / per);
+  a.tile = (int)(in % per / (u64)a.q.units);
+  a.unit = (int)(in % per % (u64)a.q.units);
+  return a;
 }
 
-// A place in the list of work.
-template <int D>
-struct KvCursor {
-  KvSeq q;
-  int s, head, tile, unit;
-
-  __device__ __forceinline__ void set(const KvAttn& p, int seq, u64 within)
-  {
-    s = seq;
-    q = kv_seq<D>(p, s);
-    const u64 per = (u64)q.tiles * (u64)q.units;
-    head = (int)(within / per);
-    const u64 r = within % per;
-    tile = (int)(r / (u64)q.units);
-    unit = (int)(r % (u64)q.units);
-  }
-  __device__ __forceinline__ void next(const KvAttn& p)
-  {
-    if (++unit < q.units) return;
-    unit = 0;
-    if (++tile < q.tiles) return;
-    tile = 0;
-    if (++head < p.kv_heads) return;
-    head = 0;
-    while (++s < p.seqs) {
-      q = kv_seq<D>(p, s);
-      if (kv_work<D>(p, q) != 0) return;
-    }
-  }
-};
+// k stages on (k at most what is left of the tile); past the list's end s
+// reaches seqs.
+template <int D, int TR, int N>
+__device__ __forceinline__ void kv_move(const KvAttn& p, const KvTable<N>& tab, KvPlace& a, int k)
+{
+  a.unit += k;
+  if (a.unit < a.q.units) return;
+  a.unit = 0;
+  if (++a.tile < a.q.tiles) return;
+  a.tile = 0;
+  if (++a.head < p.kv_heads) return;
+  a.head = 0;
+  do {
+    if (++a.s >= p.seqs) return;
+    a.q = kv_get<D, TR, N>(p, tab, a.s);
+  } while (kv_work(p, a.q) == 0);
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
 {
@@ -405,25 +444,32 @@ __device__ __forceinline__ uint32_t kv_place(int r, int ch)
   }
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t a)
+__device__ __forceinline__ uint4 lds128(const uint8_t* a)
 {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "r"(a));
-  return r;
+  return *reinterpret_cast<const uint4*>(a);
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a)
+__device__ __forceinline__ uint2 lds64(const uint8_t* a)
 {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return *reinterpret_cast<const uint2*>(a);
+}
+
+// A constant the compiler keeps in a register.
+__device__ __forceinline__ uint32_t held(uint32_t v)
+{
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
-// Bytes 0, 1 (hi = false) or 2, 3 of w, each 128 + c, as the f16 pair c.
-__device__ __forceinline__ uint32_t f16_pair(uint32_t w, bool hi)
+// Bytes 0, 1 (hi = false) or 2, 3 of w, each u = 128 + c, as the f16 pair u 2^-24.
+__device__ __forceinline__ uint32_t f16_tiny(uint32_t w, bool hi)
 {
-  const uint32_t u = __byte_perm(w, 0x64646464u, hi ? 0x4342 : 0x4140);   // 1024 + 128 + c
+  return __byte_perm(w, 0u, hi ? 0x4342 : 0x4140);
+}
+// The same bytes as the f16 pair c; k64 holds 0x64646464.
+__device__ __forceinline__ uint32_t f16_pair(uint32_t w, uint32_t k64, bool hi)
+{
+  const uint32_t u = __byte_perm(w, k64, hi ? 0x4342 : 0x4140);           // 1024 + 128 + c
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x64806480u));   // 1152
   return r;
@@ -445,464 +491,617 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
   return r;
 }
 
-// Columns of the output that lane column c holds in the accumulators' order:
-// value e of row half h (0: row g, 1: row g + 8) is O[row][kv_col(c, e)] with
-// e = w * 32 + half * 16 + j at widths 128 and 256 (128 w + 32 c + e % 32) and
-// e = half * 8 + j at 64 (16 c + e).
-template <int D>
-__device__ __forceinline__ float kv_acc(const float (&o)[D / 8][4], int h, int e)
+// Rows and columns of an 8x8 matrix of 16-bit values, a pair a lane, exchanged.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v)
 {
-  constexpr int J = D == 64 ? 8 : 16;                  // bytes of a lane's V piece
-  const int w = e / (2 * J), half = (e / J) & 1, j = e % J;
-  return o[w * J + j][h * 2 + half];
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
-template <int D>
-__global__ void __launch_bounds__(KvCfg<D>::kWarps * 32, 2)
+// The factor of a part (max m, sum l) under the joint maximum: a part that saw
+// nothing has sum 0 and O 0.
+__device__ __forceinline__ float kv_weight(float m, float l, float top)
+{
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - top);
+}
+
+// NR: groups of 8 query rows of a tile.
+template <int D, int NR>
+__global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
     kv8_attention_kernel(const __grid_constant__ KvAttn p)
 {
-  using C = KvCfg<D>;
-  constexpr int T = C::kTok, N = C::kWarps * 32;
+  using C = KvCfg<D, NR>;
+  constexpr int T = C::kTok, W = C::kWarps, N = C::kThreads, TR = 8 * NR, MT = C::kMT, OT = C::kOT;
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  __shared__ u64 s_pre[N + 1];
+  __shared__ KvTable<N> s_tab;
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   const int g = lane >> 2, cc = lane & 3;
-  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)(warp * C::kWarpBytes);
-  float4* heads = reinterpret_cast<float4*>(smem_raw + warp * C::kWarpBytes +
-                                            C::kStages * C::kStageBytes);
+  uint8_t* const mine = smem_raw + warp * 2 * C::kStageBytes;
+  const uint32_t ring = smem_u32(mine);
+  const uint32_t k64 = held(0x64646464u);
+  // This lane's places in a stage.  Pieces swizzle by bits that only the lane
+  // sets, so all of a stage is at constants from these: K row g (piece cc, and
+  // 4 + cc of 8), V rows 2 cc of 16 (piece g), the pieces it copies.
+  const uint32_t k_at[2] = {kv_place<D, false>(g, cc), kv_place<D, false>(g, D == 64 ? cc : 4 + cc)};
+  const uint32_t v_at = kv_place<D, true>(2 * cc, D == 64 ? g >> 1 : g) +
+                        (D == 64 ? (uint32_t)(g & 1) * 8u : 0u);
+  const uint32_t k_to = kv_place<D, false>(lane / (D / 16), lane % (D / 16));
+  const uint32_t v_to = kv_place<D, true>(lane / (D / 16), lane % (D / 16));
   pdl_wait();
   pdl_trigger();
-  kv_plan<D, N>(p, s_pre);
-  const u64 all = s_pre[N];
-  const u64 workers = min((u64)p.workers, all);
-  const u64 me = (u64)blockIdx.x * C::kWarps + warp;
+
+  // this warp's run of the work; neighbours in it are on different SMs
+  kv_scan<D, TR, N>(p, s_tab);
+  const u64 all = s_tab.before[N];
+  const u64 workers = kv_workers(p, all);
+  const u64 me = (u64)warp * gridDim.x + blockIdx.x;
   if (me >= workers) return;
-  const u64 begin = work_bound(all, workers, me), end = work_bound(all, workers, me + 1);
+  const u64 begin = work_bound(all, workers, me);
+  const uint32_t count = (uint32_t)(work_bound(all, workers, me + 1) - begin);
+  KvPlace at = kv_locate<D, TR, N>(p, s_tab, begin);
 
-  KvCursor<D> ld, at;
-  u64 before;
-  const int s0 = kv_find<D, N>(p, s_pre, begin, &before);
-  at.set(p, s0, begin - before);
-  ld = at;
-  // pages and scales of 32 blocks of the loading cursor's sequence and head
-  int c_s = -1, c_head = -1, c_group = -1, c_page = -1;
-  float c_ks = 0.0f, c_vs = 0.0f;
-  u64 loaded = begin;
-
-  auto load = [&](int stage) {
-    if (loaded < end) {
+  // The loading side: the next stage, and the pages of 32 blocks of its
+  // sequence, one a lane.  Scales arrive in registers two stages ahead of their
+  // use (a page that is not there is marked by an impossible one).
+  KvPlace ld = at;
+  uint32_t loaded = 0;
+  int c_s = -1, c_group = 0, c_page = -1;
+  const int8_t* v_src = nullptr;                       // values of the stage begun
+  uint32_t ks_next[2], vs_next[2];
+  auto load_k = [&](int stage, uint32_t& ks, uint32_t& vs) {
+    v_src = nullptr;
+    ks = 0xbf80u;                                      // -1
+    vs = 0;
+    if (loaded < count) {
       const int tok = (ld.q.first + ld.unit) * T;
       const int block = tok / kPage, group = block & ~31;
-      if (ld.s != c_s || ld.head != c_head || group != c_group) {
+      if (ld.s != c_s || group != c_group) {
         c_s = ld.s;
-        c_head = ld.head;
         c_group = group;
         c_page = -1;
-        if ((group + lane) * kPage < ld.q.len)
+        if ((group + lane) * kPage < ld.q.len) {
           c_page = p.table[(size_t)ld.s * p.table_ld + group + lane];
-        if (!page_ok(c_page, p.pages)) {
-          if ((group + lane) * kPage < ld.q.len) atomicCAS(p.err, 0, KERR_PLACE);
-          c_page = -1;
-        }
-        if (c_page >= 0) {
-          c_ks = bf16_bits(p.ks[(size_t)c_page * p.kv_heads + ld.head]);
-          c_vs = bf16_bits(p.vs[(size_t)c_page * p.kv_heads + ld.head]);
+          if (!page_ok(c_page, p.pages)) {
+            atomicCAS(p.err, 0, KERR_PLACE);
+            c_page = -1;
+          }
         }
       }
       const int page = __shfl_sync(0xffffffffu, c_page, block - group);
-      const float ks = __shfl_sync(0xffffffffu, c_ks, block - group);
-      const float vs = __shfl_sync(0xffffffffu, c_vs, block - group);
-      if (lane == 0) heads[stage] = make_float4(ks, vs, page < 0 ? 0.0f : 1.0f, 0.0f);
       if (page >= 0) {
-        const size_t off = ((size_t)page * p.kv_heads + ld.head) * (size_t)(kPage * D) +
-                           (size_t)(tok % kPage) * D;
-        const uint32_t dst = ring + (uint32_t)(stage * C::kStageBytes);
+        const size_t line = (size_t)page * p.kv_heads + ld.head;
+        const size_t off = line * (size_t)(kPage * D) + (size_t)(tok % kPage) * D +
+                           (size_t)lane * 16;
+        const int8_t* src = p.k + off;
+        v_src = p.v + off;
+        const uint32_t dst = ring + (uint32_t)(stage * C::kStageBytes) + k_to;
+        // piece i * 32 + lane: row i * (512 / D) further
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int x = i * 32 + lane, r = x / (D / 16), ch = x % (D / 16);
-          cp_async16(dst + kv_place<D, false>(r, ch), p.k + off + (size_t)x * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int x = i * 32 + lane, r = x / (D / 16), ch = x % (D / 16);
-          cp_async16(dst + 4096u + kv_place<D, true>(r, ch), p.v + off + (size_t)x * 16);
-        }
+        for (int i = 0; i < 8; ++i) cp_async16(dst + i * 512, src + i * 512);
+        ks = p.ks[line];
+        vs = p.vs[line];
       }
-      ++loaded;
-      ld.next(p);
+      if (++loaded < count) kv_move<D, TR, N>(p, s_tab, ld, 1);
     }
     cp_async_commit();
   };
+  auto load_v = [&](int stage) {
+    if (v_src != nullptr) {
+      const uint32_t dst = ring + (uint32_t)(stage * C::kStageBytes) + 4096u;
+      // the flip of V's rows moves with i
 #pragma unroll
-  for (int i = 0; i < C::kStages - 1; ++i) load(i);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t flip = D == 64 ? 0u : D == 128 ? (uint32_t)(i & 1) * 64u
+                                                      : (uint32_t)(i & 3) * 32u;
+        cp_async16(dst + (v_to ^ flip) + i * 512, v_src + i * 512);
+      }
+    }
+    cp_async_commit();
+  };
+  // queries of a tile as they lie: row g of each group of 8, 16 of every 64
+  // columns; rows past the tile's last are zeros, computed and never stored
+  uint4 raw[NR][D / 64][2];
+  auto fetch_q = [&]() {
+    const int row0 = at.tile * TR, rows = min(TR, at.q.n * p.group - row0);
+#pragma unroll
+    for (int h = 0; h < NR; ++h) {
+      const int r = g + 8 * h;
+      const int tok = (row0 + r) / p.group, head = at.head * p.group + (row0 + r) % p.group;
+      const __nv_bfloat16* q = p.q + (size_t)(at.q.row0 + tok) * p.ldq + (size_t)head * D;
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          raw[h][j][i] = make_uint4(0, 0, 0, 0);
+          if (r < rows) raw[h][j][i] = *reinterpret_cast<const uint4*>(q + j * 64 + cc * 16 + i * 8);
+        }
+    }
+  };
+  fetch_q();                                           // ahead of the first stages
+  load_k(0, ks_next[0], vs_next[0]);
+  load_v(0);
+  load_k(1, ks_next[1], vs_next[1]);
+  load_v(1);
 
-  uint32_t qf[D / 16][4];
-  float o[C::kOT][4];
-  float qs[2], m[2], l[2];
-  float ref = 0.0f;                                    // the scale O is held in (0: none yet)
-  int lo[2], hi[2], rr[2];
-  bool fresh = true;
   int stage = 0;
+  for (uint32_t x = 0; x < count;) {
+    // ---- a tile, or this warp's share of it
+    const uint32_t share = min((uint32_t)(at.q.units - at.unit), count - x);
+    const int row0 = at.tile * TR;
+    const int rows = min(TR, at.q.n * p.group - row0);
+    const int shift = at.q.len - at.q.n;
+    // keys that all of its rows see
+    const int all_lo = key_low(shift + (row0 + rows - 1) / p.group, p.window);
+    const int all_hi = key_high(shift + row0 / p.group, at.q.len, 1);
 
-  for (u64 x = begin; x < end; ++x) {
-    if (fresh) {
-      // a tile begins (or this worker's share of it): its queries
-      fresh = false;
-      ref = 0.0f;
+    if (x > 0) fetch_q();
+    uint32_t qf[NR][D / 16][2];
+    float qs[NR][2], qb[NR][2];                        // exponent's factor, 128 sum(q) 2^-24
 #pragma unroll
-      for (int t = 0; t < C::kOT; ++t)
+    for (int h = 0; h < NR; ++h) {
+      uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][e] = 0.0f;
+      for (int j = 0; j < D / 64; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = at.tile * kTileRows + g + 8 * h;
-        const int tok = r / p.group, head = at.head * p.group + r % p.group;
-        const bool valid = tok < at.q.n;
-        // rows past the tile's last are computed and never stored
-        rr[h] = valid ? r : -1;
-        const int pos = at.q.len - at.q.n + tok;
-        lo[h] = valid ? key_low(pos, p.window) : 0;
-        hi[h] = valid ? key_high(pos, at.q.len, 1) : INT_MAX;
-        m[h] = -INFINITY;
-        l[h] = 0.0f;
-        const __nv_bfloat16* q = p.q + (size_t)(at.q.row0 + tok) * p.ldq + (size_t)head * D;
-        uint32_t most = 0;
-        uint4 w[D / 64][2];
+        for (int i = 0; i < 2; ++i) {
+          const uint4 w = raw[h][j][i];
+          const uint32_t a = __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+          const uint32_t b = __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
+          most = __vmaxu2(most, __vmaxu2(a, b));
+        }
+      most = max(most & 0xffffu, most >> 16);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // 2^(8 - exponent of the row's largest), 1 where that is zero or not finite
+      int ex = (int)(most >> 7) - 127;
+      if (most == 0 || most > 0x7f7fu) ex = 8;
+      ex = max(ex, -100);
+      const float up = __uint_as_float((uint32_t)(127 + 8 - ex) << 23);
+      const float factor = p.c * 16777216.0f * __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
+      float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j)
+      for (int j = 0; j < D / 64; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            w[j][i] = make_uint4(0, 0, 0, 0);
-            if (valid) w[j][i] = *reinterpret_cast<const uint4*>(q + j * 64 + cc * 16 + i * 8);
-            const uint32_t a = __vmaxu2(w[j][i].x & 0x7fff7fffu, w[j][i].y & 0x7fff7fffu);
-            const uint32_t b = __vmaxu2(w[j][i].z & 0x7fff7fffu, w[j][i].w & 0x7fff7fffu);
-            most = __vmaxu2(most, __vmaxu2(a, b));
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t words[4] = {raw[h][j][i].x, raw[h][j][i].y, raw[h][j][i].z, raw[h][j][i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // 8 values of half i of the lane's 16: k steps 2 i and 2 i + 1
+            const uint32_t f = pack_f16(__uint_as_float(words[e] << 16) * up,
+                                        __uint_as_float(words[e] & 0xffff0000u) * up);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&f));
+            sum += back.x + back.y;
+            qf[h][j * 4 + i * 2 + (e >> 1)][e & 1] = f;
           }
-        most = max(most & 0xffffu, most >> 16);
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // 2^(8 - exponent of the row's largest), 1 where that is zero or not finite
-        int ex = (int)(most >> 7) - 127;
-        if (most == 0 || most > 0x7f7fu) ex = 8;
-        ex = max(ex, -100);
-        const float up = __uint_as_float((uint32_t)(127 + 8 - ex) << 23);
-        qs[h] = p.c * __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
+        }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      // scores come to this lane for rows 2 cc and 2 cc + 1
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t words[4] = {w[j][i].x, w[j][i].y, w[j][i].z, w[j][i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // 8 bf16 of piece half i: k steps 2 i and 2 i + 1
-              const float a = __uint_as_float(words[e] << 16) * up;
-              const float b = __uint_as_float(words[e] & 0xffff0000u) * up;
-              qf[j * 4 + i * 2 + (e >> 1)][(e & 1) * 2 + h] = pack_f16(a, b);
-            }
-          }
+      for (int e = 0; e < 2; ++e) {
+        qs[h][e] = __shfl_sync(0xffffffffu, factor, (2 * cc + e) * 4);
+        qb[h][e] = __shfl_sync(0xffffffffu, sum, (2 * cc + e) * 4) * 7.62939453125e-6f;
       }
     }
 
-    cp_async_wait<C::kStages - 2>();
-    __syncwarp();
-    load((stage + C::kStages - 1) % C::kStages);
-    const float4 head = heads[stage];
-    const uint32_t kb = ring + (uint32_t)(stage * C::kStageBytes), vb = kb + 4096u;
-    if (head.z != 0.0f) {
-      const int j0 = (at.q.first + at.unit) * T;
-      float sc[C::kNT][4];
+    float o[NR][OT][4];
 #pragma unroll
-      for (int t = 0; t < C::kNT; ++t) {
+    for (int h = 0; h < NR; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[t][e] = 0.0f;
+      for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[h][t][e] = 0.0f;
+    float m[NR][2], l[NR][2];
+#pragma unroll
+    for (int h = 0; h < NR; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[h][e] = -INFINITY;
+        l[h][e] = 0.0f;
+      }
+    // O is held in units of `ref`, 1/32 of a V scale met before (0: none yet)
+    float ref = 0.0f;
+
+    for (uint32_t u = 0; u < share; ++u) {
+      const uint8_t* const kb = mine + stage * C::kStageBytes;
+      const uint8_t* const vb = kb + 4096 + v_at;
+      cp_async_wait<3>();
+      __syncwarp();
+      const float ks = bf16_bits(ks_next[0]), vs = bf16_bits(vs_next[0]);
+      ks_next[0] = ks_next[1];
+      vs_next[0] = vs_next[1];
+      const bool there = ks != -1.0f;
+
+      // S^T.  A key tile's steps depend on each other: kSums sums of each keep
+      // four products in flight.
+      constexpr int kSums = MT * NR >= 4 ? 1 : 4 / (MT * NR);
+      float sc[NR][MT][kSums][4];
+#pragma unroll
+      for (int h = 0; h < NR; ++h)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int k = 0; k < kSums; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[h][t][k][e] = 0.0f;
+      if (there) {
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
-          const uint4 w = lds128(kb + kv_place<D, false>(t * 8 + g, j * 4 + cc));
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          uint4 w0[MT], w8[MT];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint32_t y = words[u] ^ 0x80808080u;
-            const uint32_t* a = qf[j * 4 + u];
-            mma_f16(sc[t], a[0], a[1], a[2], a[3], f16_pair(y, false), f16_pair(y, true));
+          for (int t = 0; t < MT; ++t) {
+            const uint8_t* row = kb + k_at[j & 1] + t * 16 * D + (j >> 1) * 128;
+            w0[t] = lds128(row);
+            w8[t] = lds128(row + 8 * D);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              const uint32_t y0 = 0x80808080u ^
+                  (i == 0 ? w0[t].x : i == 1 ? w0[t].y : i == 2 ? w0[t].z : w0[t].w);
+              const uint32_t y8 = 0x80808080u ^
+                  (i == 0 ? w8[t].x : i == 1 ? w8[t].y : i == 2 ? w8[t].z : w8[t].w);
+              const uint32_t a0 = f16_tiny(y0, false), a1 = f16_tiny(y8, false);
+              const uint32_t a2 = f16_tiny(y0, true), a3 = f16_tiny(y8, true);
+#pragma unroll
+              for (int h = 0; h < NR; ++h)
+                mma_f16(sc[h][t][i % kSums], a0, a1, a2, a3, qf[h][j * 4 + i][0],
+                        qf[h][j * 4 + i][1]);
+            }
         }
       }
-      // exponents of two: score * qs * K's scale, masked where a row does not look
-      const float f0 = qs[0] * head.x, f1 = qs[1] * head.x;
-      float mx0 = -INFINITY, mx1 = -INFINITY;
-      const bool part = j0 + T > hi[0] || j0 + T > hi[1] || j0 < lo[0] || j0 < lo[1];
-      const bool masked = __any_sync(0xffffffffu, part);
-#pragma unroll
-      for (int t = 0; t < C::kNT; ++t) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sc[t][e] *= f0;
-          sc[t][2 + e] *= f1;
-          if (masked) {
-            const int j = j0 + t * 8 + 2 * cc + e;
-            if (j < lo[0] || j >= hi[0]) sc[t][e] = -INFINITY;
-            if (j < lo[1] || j >= hi[1]) sc[t][2 + e] = -INFINITY;
-          }
-          mx0 = fmaxf(mx0, sc[t][e]);
-          mx1 = fmaxf(mx1, sc[t][2 + e]);
-        }
-      }
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      // O is held in units of `ref`, 1/32 of a V scale met before, and P carries
-      // the page's scale over it.  ref moves when that leaves [1/2, 512]: P, at
-      // most 2^kKvGrow, then stays inside f16's range and loses bits (below its
-      // normal 2^-14) only 2^13 under the row's largest
-      const float vs = head.y;
-      float fo = 1.0f;
-      if (vs > 0.0f && vs <= FLT_MAX && !(vs <= ref * 512.0f && vs >= ref * 0.5f)) {
-        fo = ref * 32.0f / vs;
-        ref = vs * 0.03125f;
-      }
-      const float ratio = ref > 0.0f ? vs / ref : vs;
-      float f[2] = {fo, fo};
-      if (mx0 > m[0] + kKvGrow) {
-        const float d = fast_exp2(m[0] - mx0);
-        m[0] = mx0;
-        l[0] *= d;
-        f[0] *= d;
-      }
-      if (mx1 > m[1] + kKvGrow) {
-        const float d = fast_exp2(m[1] - mx1);
-        m[1] = mx1;
-        l[1] *= d;
-        f[1] *= d;
-      }
-      if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
-#pragma unroll
-        for (int t = 0; t < C::kOT; ++t) {
-          o[t][0] *= f[0];
-          o[t][1] *= f[0];
-          o[t][2] *= f[1];
-          o[t][3] *= f[1];
-        }
-      }
-      const float n0 = m[0] == -INFINITY ? 0.0f : m[0], n1 = m[1] == -INFINITY ? 0.0f : m[1];
-      uint32_t pf[C::kNT][2];
-#pragma unroll
-      for (int t = 0; t < C::kNT; ++t) {
-        float pr[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          pr[e] = fast_exp2(sc[t][e] - n0);
-          pr[2 + e] = fast_exp2(sc[t][2 + e] - n1);
-        }
-        l[0] += pr[0] + pr[1];
-        l[1] += pr[2] + pr[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float w = pr[e] * ratio;
-          // a masked place stays 0 when the page's scale is not finite
-          pr[e] = masked && pr[e] == 0.0f ? 0.0f : w;
-        }
-        pf[t][0] = pack_f16(pr[0], pr[1]);
-        pf[t][1] = pack_f16(pr[2], pr[3]);
-      }
-#pragma unroll
-      for (int s = 0; s < T / 16; ++s) {
-        const int r = s * 16 + 2 * cc;
-        const uint32_t a0 = pf[2 * s][0], a1 = pf[2 * s][1];
-        const uint32_t a2 = pf[2 * s + 1][0], a3 = pf[2 * s + 1][1];
-        // four output columns from one word of each of the lane's four keys
-        auto four = [&](int base, uint32_t w0, uint32_t w1, uint32_t w8, uint32_t w9) {
-          w0 ^= 0x80808080u;
-          w1 ^= 0x80808080u;
-          w8 ^= 0x80808080u;
-          w9 ^= 0x80808080u;
-          const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
-          const uint32_t y0 = __byte_perm(w8, w9, 0x5140), y1 = __byte_perm(w8, w9, 0x7362);
-          mma_f16(o[base + 0], a0, a1, a2, a3, f16_pair(x0, false), f16_pair(y0, false));
-          mma_f16(o[base + 1], a0, a1, a2, a3, f16_pair(x0, true), f16_pair(y0, true));
-          mma_f16(o[base + 2], a0, a1, a2, a3, f16_pair(x1, false), f16_pair(y1, false));
-          mma_f16(o[base + 3], a0, a1, a2, a3, f16_pair(x1, true), f16_pair(y1, true));
-        };
-        if constexpr (D == 64) {
-          const uint32_t sub = (uint32_t)(g & 1) * 8u;
-          const uint2 w0 = lds64(vb + kv_place<D, true>(r, g >> 1) + sub);
-          const uint2 w1 = lds64(vb + kv_place<D, true>(r + 1, g >> 1) + sub);
-          const uint2 w8 = lds64(vb + kv_place<D, true>(r + 8, g >> 1) + sub);
-          const uint2 w9 = lds64(vb + kv_place<D, true>(r + 9, g >> 1) + sub);
-          four(0, w0.x, w1.x, w8.x, w9.x);
-          four(4, w0.y, w1.y, w8.y, w9.y);
-        } else {
-#pragma unroll
-          for (int w = 0; w < D / 128; ++w) {
-            const uint4 w0 = lds128(vb + kv_place<D, true>(r, w * 8 + g));
-            const uint4 w1 = lds128(vb + kv_place<D, true>(r + 1, w * 8 + g));
-            const uint4 w8 = lds128(vb + kv_place<D, true>(r + 8, w * 8 + g));
-            const uint4 w9 = lds128(vb + kv_place<D, true>(r + 9, w * 8 + g));
-            four(w * 16 + 0, w0.x, w1.x, w8.x, w9.x);
-            four(w * 16 + 4, w0.y, w1.y, w8.y, w9.y);
-            four(w * 16 + 8, w0.z, w1.z, w8.z, w9.z);
-            four(w * 16 + 12, w0.w, w1.w, w8.w, w9.w);
-          }
-        }
-      }
-    }
-    stage = (stage + 1) % C::kStages;
+      __syncwarp();
+      load_k(stage, ks_next[1], vs_next[1]);
 
-    const bool tile_end = at.unit + 1 == at.q.units;
-    if (tile_end || x + 1 == end) {
-      const u64 seg = (u64)at.unit;                    // stages of the tile before this one
-      const bool from_start = x - begin >= seg;        // this worker had the tile's first
-      constexpr int E = D / 4;                         // values of a lane's row
+      uint32_t pf[NR][MT][2];
+      if (there) {
+        const int j0 = (at.q.first + at.unit + (int)u) * T;
+        const bool masked = j0 + T > all_hi || j0 < all_lo;
+        // P carries the page's V scale over ref.  ref moves when that leaves
+        // [1/2, 512]: P, at most 2^kKvGrow, then stays inside f16's range and
+        // loses bits (below its normal 2^-14) only 2^13 under the row's largest
+        const bool usual = vs > 0.0f && vs <= FLT_MAX; // not zero, not NaN
+        float turn = 1.0f;
+        if (usual && !(vs <= ref * 512.0f && vs >= ref * 0.5f)) {
+          turn = __fdividef(ref * 32.0f, vs);
+          ref = vs * 0.03125f;
+        }
+        const float ratio = usual ? __fdividef(vs, ref) : 1.0f;
+        const float lift = __log2f(ratio), unlift = __fdividef(1.0f, ratio);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (rr[h] < 0) continue;
-        if (tile_end && from_start) {
-          const int tok = rr[h] / p.group, head_q = at.head * p.group + rr[h] % p.group;
-          __nv_bfloat16* dst = p.o + (size_t)(at.q.row0 + tok) * p.ldo + (size_t)head_q * D;
-          const bool sees = hi[h] > lo[h];
-          const float norm = (ref > 0.0f ? ref : 1.0f) / l[h];
+        for (int h = 0; h < NR; ++h) {
+          int lo[2] = {0, 0}, hi[2] = {INT_MAX, INT_MAX};
+          float s[MT][4];
 #pragma unroll
-          for (int e = 0; e < E; e += 8) {
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[t][e] = sc[h][t][0][e];
+#pragma unroll
+              for (int k = 1; k < kSums; ++k) s[t][e] += sc[h][t][k][e];
+            }
+          if (masked) {
+            // the keys each row sees
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = 8 * h + 2 * cc + e;
+              if (r < rows) {
+                const int pos = shift + (row0 + r) / p.group;
+                lo[e] = key_low(pos, p.window);
+                hi[e] = key_high(pos, at.q.len, 1);
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = j0 + t * 16 + g + (e >> 1) * 8;
+                if (j < lo[e & 1] || j >= hi[e & 1]) s[t][e] = -INFINITY;
+              }
+          }
+          // exponent of two of a score: (s - qb) * qs * K's scale
+          float f[2], n[2];
+          bool moved = turn != 1.0f;
+          float fo[2] = {turn, turn};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            f[e] = qs[h][e] * ks;
+            float mx = fmaxf(s[0][e], s[0][2 + e]);
+#pragma unroll
+            for (int t = 1; t < MT; ++t) mx = max3f(mx, s[t][e], s[t][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = mx == -INFINITY ? mx : (mx - qb[h][e]) * f[e];
+            if (mx > m[h][e] + kKvGrow) {
+              const float d = fast_exp2(m[h][e] - mx);
+              m[h][e] = mx;
+              l[h][e] *= d;
+              fo[e] *= d;
+              moved = true;
+            }
+            n[e] = fmaf(-qb[h][e], f[e], lift - (m[h][e] == -INFINITY ? 0.0f : m[h][e]));
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[h][t][e] *= fo[e & 1];
+          }
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = fast_exp2(fmaf(s[t][e], f[e & 1], n[e & 1]));
+          if (masked) {
+            // -inf * 0 is no 0: what a row does not see leaves here
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = j0 + t * 16 + g + (e >> 1) * 8;
+                if (j < lo[e & 1] || j >= hi[e & 1]) s[t][e] = 0.0f;
+              }
+          }
+          float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sum[e] += s[t][e] + s[t][2 + e];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[h][e] = fmaf(sum[e], unlift, l[h][e]);
+          if (!usual) {
+            // values of zero count in the sum alone; a NaN or an infinity reaches
+            // the rows that see the page
+            const float over = vs == 0.0f ? 0.0f : vs;
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = j0 + t * 16 + g + (e >> 1) * 8;
+                s[t][e] = j < lo[e & 1] || j >= hi[e & 1] ? 0.0f : s[t][e] * over;
+              }
+          }
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            pf[h][t][0] = transpose8(pack_f16(s[t][0], s[t][1]));
+            pf[h][t][1] = transpose8(pack_f16(s[t][2], s[t][3]));
+          }
+        }
+      }
+
+      // O^T
+      cp_async_wait<3>();
+      __syncwarp();
+      if (there) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const uint8_t* const vr = vb + t * 16 * D;
+          // four output columns from one word of each of the lane's four keys
+          auto four = [&](int base, uint32_t w0, uint32_t w1, uint32_t w8, uint32_t w9) {
+            w0 ^= 0x80808080u;
+            w1 ^= 0x80808080u;
+            w8 ^= 0x80808080u;
+            w9 ^= 0x80808080u;
+            const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
+            const uint32_t y0 = __byte_perm(w8, w9, 0x5140), y1 = __byte_perm(w8, w9, 0x7362);
+            const uint32_t a0 = f16_pair(x0, k64, false), a1 = f16_pair(x0, k64, true);
+            const uint32_t a2 = f16_pair(y0, k64, false), a3 = f16_pair(y0, k64, true);
+            const uint32_t b0 = f16_pair(x1, k64, false), b1 = f16_pair(x1, k64, true);
+            const uint32_t b2 = f16_pair(y1, k64, false), b3 = f16_pair(y1, k64, true);
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+              mma_f16(o[h][base], a0, a1, a2, a3, pf[h][t][0], pf[h][t][1]);
+              mma_f16(o[h][base + 1], b0, b1, b2, b3, pf[h][t][0], pf[h][t][1]);
+            }
+          };
+          if constexpr (D == 64) {
+            // key 2 cc + 1 is 64 bytes on in the same 128, swizzled alike
+            const uint8_t* const odd = kb + 4096 + (v_at ^ 64u) + t * 16 * D;
+            const uint2 w0 = lds64(vr), w1 = lds64(odd);
+            const uint2 w8 = lds64(vr + 8 * D), w9 = lds64(odd + 8 * D);
+            four(0, w0.x, w1.x, w8.x, w9.x);
+            four(2, w0.y, w1.y, w8.y, w9.y);
+          } else {
+#pragma unroll
+            for (int w = 0; w < D / 128; ++w) {
+              const uint4 w0 = lds128(vr + w * 128), w1 = lds128(vr + D + w * 128);
+              const uint4 w8 = lds128(vr + 8 * D + w * 128), w9 = lds128(vr + 9 * D + w * 128);
+              four(w * 8 + 0, w0.x, w1.x, w8.x, w9.x);
+              four(w * 8 + 2, w0.y, w1.y, w8.y, w9.y);
+              four(w * 8 + 4, w0.z, w1.z, w8.z, w9.z);
+              four(w * 8 + 6, w0.w, w1.w, w8.w, w9.w);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      load_v(stage);
+      stage ^= 1;
+    }
+
+    // ---- the tile's rows, or this share's part of them
+    const bool whole = at.unit == 0 && share == (uint32_t)at.q.units;
+    // a warp's first tile goes to place 0, another to 1
+    const size_t site = (me * 2 + (x == 0 ? 0 : 1)) * TR;
+    const float unit = ref > 0.0f ? ref : 1.0f;
+#pragma unroll
+    for (int h = 0; h < NR; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 4);
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 8);
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 16);
+        const int r = 8 * h + 2 * cc + e;
+        if (r >= rows) continue;
+        // this lane has columns g * 16 .. + 15 of every 128 (g * 8 .. + 7 of 64)
+        constexpr int J = D == 64 ? 4 : 8;             // tiles of a V piece
+        if (whole) {
+          const int tok = (row0 + r) / p.group, head = at.head * p.group + (row0 + r) % p.group;
+          const int pos = shift + tok;
+          const bool sees = key_high(pos, at.q.len, 1) > key_low(pos, p.window);
+          const float norm = unit / l[h][e];
+          __nv_bfloat16* dst = p.o + (size_t)(at.q.row0 + tok) * p.ldo + (size_t)head * D;
+#pragma unroll
+          for (int t = 0; t < OT; t += 4) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = sees ? pack_bf16(kv_acc<D>(o, h, e + 2 * i) * norm,
-                                      kv_acc<D>(o, h, e + 2 * i + 1) * norm)
-                          : 0u;
-            const int col = D == 64 ? cc * 16 + e : (e / 32) * 128 + cc * 32 + e % 32;
-            *reinterpret_cast<uint4*>(dst + col) = make_uint4(w[0], w[1], w[2], w[3]);
+              w[i] = sees ? pack_bf16(o[h][t + i][e] * norm, o[h][t + i][2 + e] * norm) : 0u;
+            *reinterpret_cast<uint4*>(dst + t / J * 128 + g * 2 * J + t % J * 2) =
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          // its first tile goes to place 0, its last to 1 (0 where they are one)
-          const int place = x - begin >= (u64)at.unit + 1 ? 1 : 0;
-          const size_t site = (me * 2 + place) * kTileRows + (g + 8 * h);
-          const float norm = ref > 0.0f ? ref : 1.0f;
-          float* dst = p.part_o + site * D;
+          float* dst = p.part_o + (site + r) * D;
 #pragma unroll
-          for (int e = 0; e < E; e += 4) {
-            const int col = D == 64 ? cc * 16 + e : (e / 32) * 128 + cc * 32 + e % 32;
-            *reinterpret_cast<float4*>(dst + col) =
-                make_float4(kv_acc<D>(o, h, e) * norm, kv_acc<D>(o, h, e + 1) * norm,
-                            kv_acc<D>(o, h, e + 2) * norm, kv_acc<D>(o, h, e + 3) * norm);
-          }
-          if (cc == 0) *reinterpret_cast<float2*>(p.part_ml + site * 2) = make_float2(m[h], l[h]);
+          for (int t = 0; t < OT; t += 2)
+            *reinterpret_cast<float4*>(dst + t / J * 128 + g * 2 * J + t % J * 2) =
+                make_float4(o[h][t][e] * unit, o[h][t][2 + e] * unit, o[h][t + 1][e] * unit,
+                            o[h][t + 1][2 + e] * unit);
+          if (g == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (site + r) * 2) =
+                make_float2(m[h][e], l[h][e]);
         }
       }
-      fresh = true;
-    }
-    at.next(p);
+    x += share;
+    if (x < count) kv_move<D, TR, N>(p, s_tab, at, (int)share);
   }
   cp_async_wait<0>();
 }
 
-// Joins the tiles that several workers share: with M the largest of their
-// maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Writes zeros for the
-// rows of sequences without keys, which no worker has.  A block a (row tile,
-// kv head); its warps share the parts of a row where there are many, and the
-// rows where there are few.
-constexpr int kMergeThreads = 256;
-
-template <int D>
-__global__ void __launch_bounds__(kMergeThreads) kv8_merge_kernel(const __grid_constant__ KvAttn p)
+// Joins the tiles that several warps share: with M the largest of their
+// maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, in the parts' order.
+// Writes zeros for the rows of sequences without keys, which no warp has.  A
+// block a (row tile, kv head), or each of its rows where the tiles alone leave SMs
+// idle (grid z); its warps share the rows and, where those are fewer, the parts of
+// a row.  Everything up to pdl_wait reads only what the
+// attention kernel had waited for itself.
+template <int D, int NR, int W>
+__global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant__ KvAttn p)
 {
-  constexpr int N = kMergeThreads, W = N / 32, E = D / 32;
-  __shared__ u64 s_pre[N + 1];
-  __shared__ float s_o[W][D];
+  constexpr int N = 128, E = D / 64, TR = 8 * NR;
+  __shared__ KvTable<N> s_tab;
+  __shared__ float2 s_o[W][D / 2];
   __shared__ float s_l[W];
+  const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
+  const int head = (int)blockIdx.y, slot = (int)blockIdx.x;
+  // the slot's sequence: tiles of rows are slots of cu * group rows
+  int lo = 0, hi = p.seqs;
+  if (p.seqs > N)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (slot_base(clamp_int(p.cu[mid], 0, p.rows) * p.group, mid, TR, 1) <= slot) lo = mid;
+      else hi = mid;
+    }
+  kv_scan<D, TR, N>(p, s_tab);
+  if (p.seqs <= N)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (slot_base(s_tab.q[mid].row0 * p.group, mid, TR, 1) <= slot) lo = mid;
+      else hi = mid;
+    }
+  const int s = lo;
+  const KvSeq q = kv_get<D, TR, N>(p, s_tab, s);
+  const int tile = slot - slot_base(q.row0 * p.group, s, TR, 1);
+  int rows = tile < 0 || tile >= q.tiles ? 0 : min(TR, q.n * p.group - tile * TR);
+  // this block's rows: r_from .. rows - 1
+  const int r_from = (int)blockIdx.z * (TR / (int)gridDim.z);
+  rows = min(rows, r_from + TR / (int)gridDim.z);
+  const u64 all = s_tab.before[N], workers = kv_workers(p, all);
+  const int each = (p.seqs + N - 1) / N;
+  u64 at = s_tab.before[s / each];
+  for (int i = s / each * each; i < s; ++i) at += kv_work(p, kv_get<D, TR, N>(p, s_tab, i));
+  at += ((u64)head * q.tiles + tile) * (u64)q.units;
+  u64 first = 0, last = 0, place0 = 0;
+  if (rows > r_from && q.units > 0) {
+    first = work_owner(all, workers, at);
+    last = work_owner(all, workers, at + q.units - 1);
+    place0 = work_bound(all, workers, first) < at ? 1 : 0;
+  }
   pdl_wait();
   pdl_trigger();
-  const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
-  const int head = (int)blockIdx.y;
-  const int slot = (int)blockIdx.x;
-  // tiles of rows are slots of cu * group rows
-  int lo = 0, hi = p.seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (slot_base(clamp_int(p.cu[mid], 0, p.rows) * p.group, mid, kTileRows, 1) <= slot) lo = mid;
-    else hi = mid;
-  }
-  const int s = lo;
-  const KvSeq q = kv_seq<D>(p, s);
-  const int tile = slot - slot_base(q.row0 * p.group, s, kTileRows, 1);
-  if (tile < 0 || tile >= q.tiles) return;
-  const int rows = min(kTileRows, q.n * p.group - tile * kTileRows);
+  if (rows <= r_from) return;
   if (q.units == 0) {
-    for (int i = (int)threadIdx.x; i < rows * D; i += N) {
-      const int r = tile * kTileRows + i / D;
+    for (int i = r_from * D + (int)threadIdx.x; i < rows * D; i += W * 32) {
+      const int r = tile * TR + i / D;
       p.o[(size_t)(q.row0 + r / p.group) * p.ldo + (size_t)(head * p.group + r % p.group) * D +
           i % D] = __float2bfloat16_rn(0.0f);
     }
     return;
   }
-  kv_plan<D, N>(p, s_pre);
-  const u64 all = s_pre[N];
-  const u64 workers = min((u64)p.workers, all);
-  // the work before this sequence
-  const int each = (p.seqs + N - 1) / N;
-  u64 at = s_pre[s / each];
-  for (int i = s / each * each; i < s; ++i) at += kv_work<D>(p, kv_seq<D>(p, i));
-  at += ((u64)head * q.tiles + tile) * (u64)q.units;
-  const u64 first = work_owner(all, workers, at);
-  const u64 last = work_owner(all, workers, at + q.units - 1);
-  if (first == last) return;                           // written by its worker
+  if (first == last) return;                           // written by its warp
   const int parts = (int)(last - first) + 1;
-  const u64 place0 = work_bound(all, workers, first) < at ? 1 : 0;
-  auto site = [&](int i, int r) {
-    return ((first + i) * 2 + (i == 0 ? place0 : 0)) * kTileRows + r;
-  };
-  const bool few = parts <= W;                         // a warp a row
-  for (int r0 = 0; r0 < rows; r0 += few ? W : 1) {
-    const int r = few ? r0 + warp : r0;
-    const bool active = r < rows;
-    float M = -INFINITY;
-    if (active)
-      for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_ml[site(i, r) * 2]);
-    for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-    float acc[E], l = 0.0f;
+  auto site = [&](int i, int r) { return ((first + i) * 2 + (i == 0 ? place0 : 0)) * TR + r; };
+  // `wide` warps a row, a power of two
+  const int own = rows - r_from;
+  const int wide = max(1, W / (own > 8 ? 16 : own > 4 ? 8 : own > 2 ? 4 : own > 1 ? 2 : 1));
+  for (int r0 = r_from; r0 < rows; r0 += W / wide) {
+    const int r = r0 + warp / wide, mine = warp % wide;
+    float2 acc[E];
+    float l = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    if (active) {
+    for (int e = 0; e < E; ++e) acc[e] = make_float2(0.0f, 0.0f);
+    if (r < rows) {
+      // 32 parts' factors at a time, one a lane; the first batch of each warp has
+      // no maximum to wait for but its own
+      float top = -INFINITY;
 #pragma unroll 4
-      for (int i = few ? 0 : warp; i < parts; i += few ? 1 : W) {
-        const u64 at_i = site(i, r);
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at_i * 2);
-        // a part that saw nothing has sum 0 and O 0
-        const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : fast_exp2(ml.x - M);
-        l = fmaf(f, ml.y, l);
-        const float* src = p.part_o + at_i * D;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, src[e * 32 + lane], acc[e]);
-      }
-    }
-    if (!few) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
-      if (lane == 0) s_l[warp] = l;
-      __syncthreads();
-    }
-    const int rt = tile * kTileRows + r;
-    const int tok = rt / p.group, pos = q.len - q.n + tok;
-    const bool sees = key_high(pos, q.len, 1) > key_low(pos, p.window);
-    __nv_bfloat16* dst = p.o + (size_t)(q.row0 + tok) * p.ldo +
-                         (size_t)(head * p.group + rt % p.group) * D;
-    if (few) {
-      if (active)
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          dst[e * 32 + lane] = __float2bfloat16_rn(sees ? acc[e] / l : 0.0f);
-    } else {
-      for (int d = (int)threadIdx.x; d < D; d += N) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          a += s_o[w][d];
-          b += s_l[w];
+      for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[site(i, r) * 2]);
+      for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const int per = (parts + wide - 1) / wide;       // this warp: parts [mine per, ...)
+      const int end = min(parts, (mine + 1) * per);
+      for (int i0 = mine * per; i0 < end; i0 += 32) {
+        float f = 0.0f;
+        if (i0 + lane < end) {
+          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + site(i0 + lane, r) * 2);
+          f = kv_weight(ml.x, ml.y, top);
+          l = fmaf(f, ml.y, l);
         }
-        dst[d] = __float2bfloat16_rn(sees ? a / b : 0.0f);
+        const int n = min(32, end - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float fi = __shfl_sync(0xffffffffu, f, i);
+          const float2* src = reinterpret_cast<const float2*>(p.part_o + site(i0 + i, r) * D) + lane;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float2 v = src[e * 32];
+            acc[e].x = fmaf(fi, v.x, acc[e].x);
+            acc[e].y = fmaf(fi, v.y, acc[e].y);
+          }
+        }
+      }
+      for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    }
+    if (wide > 1) {
+      if (r < rows) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
+        if (lane == 0) s_l[warp] = l;
       }
       __syncthreads();
+      if (r < rows && mine == 0)
+        for (int w = 1; w < wide; ++w) {
+          l += s_l[warp + w];
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float2 v = s_o[warp + w][e * 32 + lane];
+            acc[e].x += v.x;
+            acc[e].y += v.y;
+          }
+        }
+    }
+    if (r < rows && mine == 0) {
+      const int rt = tile * TR + r;
+      const int tok = rt / p.group, pos = q.len - q.n + tok;
+      const bool sees = key_high(pos, q.len, 1) > key_low(pos, p.window);
+      const float norm = 1.0f / l;
+      __nv_bfloat16* dst = p.o + (size_t)(q.row0 + tok) * p.ldo +
+                           (size_t)(head * p.group + rt % p.group) * D;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        *reinterpret_cast<uint32_t*>(dst + (e * 32 + lane) * 2) =
+            sees ? pack_bf16(acc[e].x * norm, acc[e].y * norm) : 0u;
     }
   }
 }
@@ -932,10 +1131,10 @@ dim3 kv_pages_grid(const Kv8Cache& c, const Kv8Rows& r)
   return dim3((unsigned)slot_count(r.rows, r.seqs, kPage, 2), (unsigned)c.kv_heads, 2);
 }
 
-template <int D>
+template <int D, int NR>
 int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
 {
-  using C = KvCfg<D>;
+  using C = KvCfg<D, NR>;
   KvAttn p;
   memset(&p, 0, sizeof(p));
   p.k = a.cache.k;
@@ -958,21 +1157,38 @@ int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
   p.window = a.window;
   p.c = a.scale * 1.4426950408889634f;
   p.err = err;
-  const int slots = slot_count(p.rows * p.group, p.seqs, kTileRows, 1);
-  // two blocks an SM, fewer where the longest sequences cannot fill them
+  const int slots = slot_count(p.rows * p.group, p.seqs, 8 * NR, 1);
+  // a block for each SM, fewer where the longest sequences cannot fill them
   const long long units = (long long)slots * p.kv_heads * ((a.max_len + C::kTok - 1) / C::kTok + 1);
-  const long long blocks = (units + C::kWarps - 1) / C::kWarps;
-  const int grid = (int)(blocks < 2 * num_sms ? (blocks < 1 ? 1 : blocks) : 2 * num_sms);
+  const int grid = (int)(units < num_sms ? (units < 1 ? 1 : units) : num_sms);
   p.workers = grid * C::kWarps;
   p.part_o = a.workspace;
-  p.part_ml = a.workspace + (size_t)p.workers * 2 * kTileRows * D;
+  p.part_ml = p.part_o + (size_t)p.workers * 2 * (8 * NR) * D;
   static std::atomic<unsigned long long> attr{0};
-  if (!smem_limit_once(kv8_attention_kernel<D>, C::kSmem, attr)) return -1;
-  launch_k(kv8_attention_kernel<D>, dim3((unsigned)grid), dim3(C::kWarps * 32), C::kSmem, s, 1, p);
+  if (!smem_limit_once(kv8_attention_kernel<D, NR>, C::kSmem, attr)) return -1;
+  launch_k(kv8_attention_kernel<D, NR>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1, p);
   if (launched() != 0) return -1;
-  launch_k(kv8_merge_kernel<D>, dim3((unsigned)slots, (unsigned)p.kv_heads), dim3(kMergeThreads), 0,
-           s, 1, p);
+  // few tiles have many parts each: 32 warps a row; else a warp a row
+  if ((long long)slots * p.kv_heads * 2 <= num_sms)
+    launch_k(kv8_merge_kernel<D, NR, 32>, dim3((unsigned)slots, (unsigned)p.kv_heads, 8 * NR),
+             dim3(1024), 0, s, 1, p);
+  else if ((long long)p.rows * p.group > 4ll * p.seqs)
+    launch_k(kv8_merge_kernel<D, NR, 8>, dim3((unsigned)slots, (unsigned)p.kv_heads), dim3(256), 0,
+             s, 1, p);
+  else
+    launch_k(kv8_merge_kernel<D, NR, 4>, dim3((unsigned)slots, (unsigned)p.kv_heads), dim3(128), 0,
+             s, 1, p);
   return launched();
+}
+
+// Tiles of 8 rows where the sequences have no more on the average (a decoded
+// token under up to 8 query heads a key head), else of 16.
+template <int D>
+int kv_attn_tiles(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
+{
+  const long long rows = (long long)a.rows.rows * (a.heads / a.cache.kv_heads);
+  return rows <= 8ll * a.rows.seqs ? kv_attn_launch<D, 1>(a, num_sms, err, s)
+                                   : kv_attn_launch<D, 2>(a, num_sms, err, s);
 }
 
 }  // namespace
@@ -1007,15 +1223,20 @@ int launch_kv8_read(const Kv8Cache& c, const Kv8Rows& r, __nv_bfloat16* k, int l
 
 size_t kv8_attention_workspace(int head_dim, int num_sms)
 {
-  return (size_t)(2 * num_sms) * 4 * 2 * kTileRows * (size_t)(head_dim + 2) * sizeof(float);
+  // the larger of the two tile heights at the width (12 warps x 8 rows at most
+  // beside 8 x 16)
+  const size_t rows = (size_t)num_sms * 2 * 16 * KvCfg<128, 2>::kWarps;
+  static_assert(KvCfg<128, 1>::kWarps * 8 <= KvCfg<128, 2>::kWarps * 16 &&
+                KvCfg<256, 2>::kWarps == KvCfg<128, 2>::kWarps, "rows of the workspace");
+  return rows * (size_t)(head_dim + 2) * sizeof(float);
 }
 
 int launch_kv8_attention(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
 {
   switch (a.cache.head_dim) {
-    case 64: return kv_attn_launch<64>(a, num_sms, err, s);
-    case 128: return kv_attn_launch<128>(a, num_sms, err, s);
-    case 256: return kv_attn_launch<256>(a, num_sms, err, s);
+    case 64: return kv_attn_tiles<64>(a, num_sms, err, s);
+    case 128: return kv_attn_tiles<128>(a, num_sms, err, s);
+    case 256: return kv_attn_tiles<256>(a, num_sms, err, s);
     default: return -2;
   }
 }

@@ -195,6 +195,15 @@ class Context:
         self.h = h
         self.device = device
 
+    @property
+    def torch_device(self):
+        """The context's device as torch names it."""
+        d = self.__dict__.get("_torch_device")
+        if d is None:
+            import torch
+            d = self._torch_device = torch.device("cuda", self.device)
+        return d
+
     def close(self):
         if getattr(self, "h", None) is not None and self.h.value:
             self.lib.ltx_ctx_destroy(self.h)
@@ -756,6 +765,8 @@ def attention(ctx, q, k, v, heads, head_dim, gate=None, tq=None, tk=None,
 
 
 # ---- the caption language model -------------------------------------------------
+# A served token costs a few microseconds on the GPU, so these wrappers check with
+# as few calls into torch as will do and build messages only to raise them.
 
 
 def _stream_of(ctx, stream):
@@ -763,46 +774,67 @@ def _stream_of(ctx, stream):
     device unless one is given."""
     if stream is None:
         import torch
-        return ctypes.c_void_p(torch.cuda.current_stream(ctx.device).cuda_stream)
-    return _stream(stream)
+        return torch._C._cuda_getCurrentRawStream(ctx.device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _new_on(ctx, stream, make):
-    """make() with allocations ordered on the call's stream."""
+def _new(ctx, stream, shape, dtype):
+    """A tensor on the context's device, allocated in the order of the call's stream."""
     import torch
     if stream is None:
-        return make()
-    s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+        return torch.empty(shape, dtype=dtype, device=ctx.torch_device)
+    s = torch.cuda.ExternalStream(stream, ctx.torch_device) if isinstance(stream, int) else stream
     with torch.cuda.stream(s):
-        return make()
+        return torch.empty(shape, dtype=dtype, device=ctx.torch_device)
 
 
-def _need(ok, code, what):
-    if not ok:
-        raise LtxError(code, what)
+def _elsewhere(ctx, t, name):
+    return LtxError(-2, f"{name}: need a tensor on cuda:{ctx.device}, got {t.device}")
 
 
-def _rows(ctx, t, cols, name):
-    """A [rows][cols] bf16 tensor on the context's device with adjacent columns."""
+def _rows(ctx, t, cols, name, rows=None):
+    """The row stride of a [rows][cols] bf16 tensor on the context's device with
+    adjacent columns."""
     import torch
-    _need(t.dtype == torch.bfloat16, -3, f"{name}: need bfloat16, got {t.dtype}")
-    _need(t.dim() == 2 and t.shape[1] == cols and (t.stride(1) == 1 or t.shape[0] == 0), -2,
-          f"{name}: need [rows][{cols}] with adjacent columns, got {tuple(t.shape)}")
-    _need(t.device.type == "cuda" and t.device.index == ctx.device, -2,
-          f"{name}: need a tensor on cuda:{ctx.device}, got {t.device}")
-    # one row (or none) has no stride to speak of; a broadcast one stays as it is,
-    # and is refused
-    return t.stride(0) if t.shape[0] > 1 else (cols + 7) // 8 * 8
+    if t.dtype is not torch.bfloat16:
+        raise LtxError(-3, f"{name}: need bfloat16, got {t.dtype}")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+        raise LtxError(-2, f"{name}: need [{'rows' if rows is None else rows}][{cols}], got "
+                           f"{tuple(shape)}")
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, t, name)
+    if shape[0] < 2:                     # one row (or none) has no stride to speak of
+        if shape[0] == 1 and t.stride(1) != 1:
+            raise LtxError(-2, f"{name}: need adjacent columns")
+        return (cols + 7) // 8 * 8
+    ld, one = t.stride()
+    if one != 1 or ld < cols:            # broadcast rows too
+        raise LtxError(-2, f"{name}: need adjacent columns and rows that do not overlap, got "
+                           f"strides {t.stride()}")
+    return ld
 
 
 def _ints(ctx, t, n, name):
-    """A contiguous int32 tensor of n values on the context's device."""
+    """The address of n adjacent int32 values on the context's device."""
     import torch
-    _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n, -2,
-          f"{name}: need {n} adjacent int32 values, got {tuple(t.shape)} {t.dtype}")
-    _need(t.device.type == "cuda" and t.device.index == ctx.device, -2,
-          f"{name}: need a tensor on cuda:{ctx.device}, got {t.device}")
-    return _ptr(t)
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise LtxError(-2, f"{name}: need {n} adjacent int32 values, got {tuple(t.shape)} "
+                           f"{t.dtype}")
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, t, name)
+    return t.data_ptr()
+
+
+def _table(ctx, t, seqs):
+    """The address and columns of a page table, int32 [seqs][columns]."""
+    import torch
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != seqs or not t.is_contiguous():
+        raise LtxError(-2, f"table: need contiguous int32 [{seqs}][columns], got "
+                           f"{tuple(t.shape)} {t.dtype}")
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, t, "table")
+    return t.data_ptr(), t.shape[1]
 
 
 def attention_packed(ctx, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal=True, window=0,
@@ -812,24 +844,23 @@ def attention_packed(ctx, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal
     are fine), cu_q and cu_k int32 [seqs + 1] on the device.  scale: 1/sqrt(D) by
     default.  Returns [rows][heads * D]; rows outside the sequences are left as
     they are in `out`."""
-    import torch
-    seqs = cu_q.numel() - 1
-    ldq = _rows(ctx, q, heads * head_dim, "q")
+    seqs, rows, keys = cu_q.numel() - 1, q.shape[0], k.shape[0]
+    cols = heads * head_dim
+    ldq = _rows(ctx, q, cols, "q")
     ldk = _rows(ctx, k, kv_heads * head_dim, "k")
-    ldv = _rows(ctx, v, kv_heads * head_dim, "v")
-    _need(k.shape[0] == v.shape[0], -2, "attention_packed: k and v differ in rows")
-    pq, pk = _ints(ctx, cu_q, seqs + 1, "cu_q"), _ints(ctx, cu_k, seqs + 1, "cu_k")
-    rows = q.shape[0]
+    ldv = _rows(ctx, v, kv_heads * head_dim, "v", keys)
+    pq = _ints(ctx, cu_q, seqs + 1, "cu_q")
+    pk = pq if cu_k is cu_q else _ints(ctx, cu_k, seqs + 1, "cu_k")
     if out is None:
-        out = _new_on(ctx, stream, lambda: torch.empty((rows, heads * head_dim), dtype=q.dtype,
-                                                       device=q.device))
-    ldo = _rows(ctx, out, heads * head_dim, "out")
-    _need(out.shape[0] == rows, -2, "attention_packed: out and q differ in rows")
-    ctx._ok(ctx.lib.ltx_attention_packed(
-        ctx.h, _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out), ldo, pq, pk, seqs, rows,
-        k.shape[0], heads, kv_heads, head_dim, int(causal), window,
-        head_dim ** -0.5 if scale is None else scale, _stream_of(ctx, stream)),
-        "attention_packed")
+        out, ldo = _new(ctx, stream, (rows, cols), q.dtype), cols
+    else:
+        ldo = _rows(ctx, out, cols, "out", rows)
+    rc = ctx.lib.ltx_attention_packed(
+        ctx.h, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, pq,
+        pk, seqs, rows, keys, heads, kv_heads, head_dim, causal, window,
+        head_dim ** -0.5 if scale is None else scale, _stream_of(ctx, stream))
+    if rc != LTX_OK:
+        ctx._ok(rc, "attention_packed")
     return out
 
 
@@ -848,78 +879,77 @@ class KV8Cache:
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch
-        _need(k.dim() == 4 and k.shape[2] == self.PAGE and k.shape == v.shape, -2,
-              f"KV8Cache: need codes [pages][kv_heads][64][head_dim], got {tuple(k.shape)} and "
-              f"{tuple(v.shape)}")
-        self.pages, self.kv_heads, _, self.head_dim = k.shape
-        for t, dt, shape in ((k, torch.int8, k.shape), (v, torch.int8, k.shape),
-                             (k_scale, torch.bfloat16, k.shape[:2]),
-                             (v_scale, torch.bfloat16, k.shape[:2])):
-            _need(t.dtype == dt and t.shape == shape and t.is_contiguous() and
-                  t.device == k.device, -2,
-                  f"KV8Cache: need a contiguous {dt} tensor {tuple(shape)} on {k.device}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != self.PAGE:
+            raise LtxError(-2, "KV8Cache: need codes [pages][kv_heads][64][head_dim], got "
+                               f"{tuple(shape)}")
+        dev, few = k.get_device(), shape[:2]
+        if k.dtype is not torch.int8 or v.dtype is not torch.int8 or \
+                k_scale.dtype is not torch.bfloat16 or v_scale.dtype is not torch.bfloat16 or \
+                v.shape != shape or k_scale.shape != few or v_scale.shape != few or \
+                not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and
+                     v_scale.is_contiguous()) or \
+                v.get_device() != dev or k_scale.get_device() != dev or \
+                v_scale.get_device() != dev:
+            raise LtxError(-2, f"KV8Cache: need contiguous int8 codes {tuple(shape)} and bfloat16 "
+                               f"scales {tuple(few)} on one device")
+        self.pages, self.kv_heads, _, self.head_dim = shape
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, dev
         self._c = _KV8Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                              self.pages, self.kv_heads, self.head_dim)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def empty(cls, ctx, pages, kv_heads, head_dim):
         import torch
-        dev = torch.device("cuda", ctx.device)
         codes = (pages, kv_heads, cls.PAGE, head_dim)
-        return cls(torch.empty(codes, dtype=torch.int8, device=dev),
-                   torch.empty(codes, dtype=torch.int8, device=dev),
-                   torch.empty(codes[:2], dtype=torch.bfloat16, device=dev),
-                   torch.empty(codes[:2], dtype=torch.bfloat16, device=dev))
+        new = lambda shape, dtype: torch.empty(shape, dtype=dtype,             # noqa: E731
+                                               device=ctx.torch_device)
+        return cls(new(codes, torch.int8), new(codes, torch.int8),
+                   new(codes[:2], torch.bfloat16), new(codes[:2], torch.bfloat16))
 
     def _on(self, ctx):
-        d = self.k.device
-        _need(d.type == "cuda" and d.index == ctx.device, -2,
-              f"KV8Cache: need a cache on cuda:{ctx.device}, got {d}")
-        return ctypes.byref(self._c)
-
-
-def _table(ctx, table, seqs):
-    import torch
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == seqs and
-          table.is_contiguous(), -2,
-          f"table: need contiguous int32 [{seqs}][columns], got {tuple(table.shape)} {table.dtype}")
-    _need(table.device.type == "cuda" and table.device.index == ctx.device, -2,
-          f"table: need a tensor on cuda:{ctx.device}, got {table.device}")
-    return _ptr(table), table.shape[1]
+        if self.device != ctx.device:
+            raise _elsewhere(ctx, self.k, "KV8Cache")
+        return self._ref
 
 
 def kv8_append(ctx, cache, k, v, cu, starts, table, stream=None):
     """ltx_kv8_append: rows cu[s] + i of k and v [rows][kv_heads * head_dim] (bf16)
     become tokens starts[s] + i of sequence s.  cu int32 [seqs + 1], starts int32
     [seqs], table int32 [seqs][columns], all on the device."""
-    seqs, cols = cu.numel() - 1, cache.kv_heads * cache.head_dim
-    ldk, ldv = _rows(ctx, k, cols, "k"), _rows(ctx, v, cols, "v")
-    _need(k.shape[0] == v.shape[0], -2, "kv8_append: k and v differ in rows")
+    seqs, rows, cols = cu.numel() - 1, k.shape[0], cache.kv_heads * cache.head_dim
+    ldk, ldv = _rows(ctx, k, cols, "k"), _rows(ctx, v, cols, "v", rows)
     pt, tld = _table(ctx, table, seqs)
-    ctx._ok(ctx.lib.ltx_kv8_append(
-        ctx.h, cache._on(ctx), _ptr(k), ldk, _ptr(v), ldv, _ints(ctx, cu, seqs + 1, "cu"),
-        _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, k.shape[0], _stream_of(ctx, stream)),
-        "kv8_append")
+    rc = ctx.lib.ltx_kv8_append(
+        ctx.h, cache._on(ctx), k.data_ptr(), ldk, v.data_ptr(), ldv,
+        _ints(ctx, cu, seqs + 1, "cu"), _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, rows,
+        _stream_of(ctx, stream))
+    if rc != LTX_OK:
+        ctx._ok(rc, "kv8_append")
 
 
 def kv8_read(ctx, cache, cu, starts, table, rows, k=None, v=None, stream=None):
     """ltx_kv8_read: tokens starts[s] + i of the sequences back as bf16 rows
     cu[s] + i of k and v [rows][kv_heads * head_dim] (new tensors by default);
     returns (k, v)."""
-    import torch
     seqs, cols = cu.numel() - 1, cache.kv_heads * cache.head_dim
-    make = lambda: torch.empty((rows, cols), dtype=torch.bfloat16,             # noqa: E731
-                               device=cache.k.device)
-    k = _new_on(ctx, stream, make) if k is None else k
-    v = _new_on(ctx, stream, make) if v is None else v
-    ldk, ldv = _rows(ctx, k, cols, "k"), _rows(ctx, v, cols, "v")
-    _need(k.shape[0] == rows and v.shape[0] == rows, -2, "kv8_read: k and v need `rows` rows")
+    bf16 = cache.k_scale.dtype
+    if k is None:
+        k, ldk = _new(ctx, stream, (rows, cols), bf16), cols
+    else:
+        ldk = _rows(ctx, k, cols, "k", rows)
+    if v is None:
+        v, ldv = _new(ctx, stream, (rows, cols), bf16), cols
+    else:
+        ldv = _rows(ctx, v, cols, "v", rows)
     pt, tld = _table(ctx, table, seqs)
-    ctx._ok(ctx.lib.ltx_kv8_read(
-        ctx.h, cache._on(ctx), _ptr(k), ldk, _ptr(v), ldv, _ints(ctx, cu, seqs + 1, "cu"),
-        _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, rows, _stream_of(ctx, stream)),
-        "kv8_read")
+    rc = ctx.lib.ltx_kv8_read(
+        ctx.h, cache._on(ctx), k.data_ptr(), ldk, v.data_ptr(), ldv,
+        _ints(ctx, cu, seqs + 1, "cu"), _ints(ctx, starts, seqs, "starts"), pt, tld, seqs, rows,
+        _stream_of(ctx, stream))
+    if rc != LTX_OK:
+        ctx._ok(rc, "kv8_read")
     return k, v
 
 
@@ -937,28 +967,29 @@ def kv8_attention(ctx, cache, q, cu_q, lengths, table, heads, max_len, window=0,
     tokens of sequences whose lengths[s] tokens the cache holds, over those tokens.
     scale: 1/sqrt(head_dim) by default; workspace: a device tensor of
     kv8_attention_workspace bytes (a new one by default; calls that may overlap
-    need one each).  Returns [rows][heads * head_dim]."""
-    import torch
-    seqs, D = cu_q.numel() - 1, cache.head_dim
-    rows = q.shape[0]
-    ldq = _rows(ctx, q, heads * D, "q")
+    need one each, and a captured call keeps the address of the one it was given).
+    Returns [rows][heads * head_dim]."""
+    seqs, rows, D = cu_q.numel() - 1, q.shape[0], cache.head_dim
+    cols = heads * D
+    ldq = _rows(ctx, q, cols, "q")
     if out is None:
-        out = _new_on(ctx, stream, lambda: torch.empty((rows, heads * D), dtype=q.dtype,
-                                                       device=q.device))
-    ldo = _rows(ctx, out, heads * D, "out")
-    _need(out.shape[0] == rows, -2, "kv8_attention: out and q differ in rows")
+        out, ldo = _new(ctx, stream, (rows, cols), q.dtype), cols
+    else:
+        ldo = _rows(ctx, out, cols, "out", rows)
     pt, tld = _table(ctx, table, seqs)
     if workspace is None:
-        need = kv8_attention_workspace(ctx, D)
-        workspace = _new_on(ctx, stream, lambda: torch.empty(need, dtype=torch.uint8,
-                                                             device=q.device))
-    _need(workspace.device == q.device and workspace.is_contiguous(), -2,
-          f"workspace: need a contiguous tensor on {q.device}")
-    ctx._ok(ctx.lib.ltx_kv8_attention(
-        ctx.h, cache._on(ctx), _ptr(q), ldq, _ptr(out), ldo, _ints(ctx, cu_q, seqs + 1, "cu_q"),
-        _ints(ctx, lengths, seqs, "lengths"), pt, tld, seqs, rows, heads, max_len, window,
-        D ** -0.5 if scale is None else scale, _ptr(workspace),
-        workspace.numel() * workspace.element_size(), _stream_of(ctx, stream)), "kv8_attention")
+        import torch
+        workspace = _new(ctx, stream, kv8_attention_workspace(ctx, D), torch.uint8)
+    elif workspace.get_device() != ctx.device or not workspace.is_contiguous():
+        raise LtxError(-2, f"workspace: need a contiguous tensor on cuda:{ctx.device}")
+    rc = ctx.lib.ltx_kv8_attention(
+        ctx.h, cache._on(ctx), q.data_ptr(), ldq, out.data_ptr(), ldo,
+        _ints(ctx, cu_q, seqs + 1, "cu_q"), _ints(ctx, lengths, seqs, "lengths"), pt, tld, seqs,
+        rows, heads, max_len, window, D ** -0.5 if scale is None else scale,
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream_of(ctx, stream))
+    if rc != LTX_OK:
+        ctx._ok(rc, "kv8_attention")
     return out
 
 
