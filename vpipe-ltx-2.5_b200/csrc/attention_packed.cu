@@ -12,14 +12,22 @@
 // (row = token * G + head, one 3-D TMA box), so K and V are read once for the
 // group and a causal tile ends TQ tokens, not 128, past its first row.
 //
-// A CTA holds two query tiles (head widths 64 and 128) or one (256: its O
-// takes 256 of the 512 TMEM columns), the layout of attention_tc.cu:
+// A CTA holds four query tiles of 64-key steps (head width 64), two of 128-key
+// steps (128) or one (256: its O takes 256 of the 512 TMEM columns), the layout
+// of attention_tc.cu:
 //   warp 0      TMA: Q, then K and V tiles in the order the MMAs use them,
 //               through one ring of equal slots
 //   warp 1      MMA: S = Q K^T, O += P V with P read from TMEM
-//   warps 4-..  softmax, eight warps a query tile, two for each TMEM lane
-//               quarter (64 score columns each)
-// With two tiles one's MMAs run under the other's softmax; with one tile the
+//   warp 2      takes work: finds an item's sequence and keys and hands them to
+//               the others through shared memory, one item ahead
+//   warps 4-..  softmax, 64 score columns a thread: eight warps a query tile,
+//               two for each TMEM lane quarter, or four with a row a thread
+// An item is a CTA's query tiles of one key head.  The grid has a CTA
+// for each; a CTA that runs takes over the next one not yet launched (cluster
+// launch control), so that barriers and TMEM are set up once, the next item's
+// loads and first scores run under this one's last softmax and store, and the
+// items, longest first in a causal sequence, go to whoever is free.
+// With several tiles one's MMAs run under the others' softmax; with one tile the
 // scores are double-buffered, so S of key tile j + 1 runs under softmax j.
 // V is used as TMA lays it down, [key][64 dims] in 128-byte swizzled rows: the
 // MN-major form of the MMA's B operand, no transposed copy.
@@ -49,7 +57,6 @@ namespace ltx {
 namespace {
 
 constexpr int kRows = 128;        // query rows of a tile = TMEM lanes
-constexpr int kKeys = 128;        // keys of a tile
 constexpr float kGrow = 8.0f;     // log2 of the largest P before O is rescaled
 
 enum : int {
@@ -57,28 +64,34 @@ enum : int {
   PERR_MMA = 0x66,
   PERR_SOFTMAX = 0x67,
   PERR_DRAIN = 0x68,
+  PERR_ITEM = 0x6A,
 };
 
 template <int D>
 struct PkCfg {
-  static constexpr int kTiles = D == 256 ? 1 : 2;      // query tiles of a CTA
-  static constexpr int kThreads = 128 + 256 * kTiles;
-  static constexpr int kAtom = 128 * 128;              // 128 rows x 128 B (64 dims)
-  static constexpr int kQTile = (D / 64) * kAtom;
+  static constexpr int kTiles = D == 64 ? 4 : D == 128 ? 2 : 1;   // query tiles of a CTA
+  static constexpr int kKeys = D == 64 ? 64 : 128;     // keys of a tile
+  static constexpr int kSplit = kKeys / 64;            // softmax threads of a row
+  static constexpr int kGroup = 4 * kSplit;            // softmax warps of a query tile
+  static constexpr int kThreads = 128 + 32 * kGroup * kTiles;
+  static constexpr int kQAtom = kRows * 128;           // 128 rows x 128 B (64 dims)
+  static constexpr int kQTile = (D / 64) * kQAtom;
   // One ring slot: a K or V tile, or half of one at width 256 (K: 128 dims
   // of 128 keys; V: all dims of 64 keys).
   static constexpr int kParts = D == 256 ? 2 : 1;
-  static constexpr int kSlot = (D / 64) * kAtom / kParts;
-  static constexpr int kSlots = D == 64 ? 8 : (D == 128 ? 4 : 5);
+  static constexpr int kKAtom = kKeys * 128;
+  static constexpr int kSlot = (D / 64) * kKAtom / kParts;
+  static constexpr int kSlots = D == 64 ? 16 : (D == 128 ? 4 : 5);
   static constexpr int kVKeys = kKeys / kParts;        // keys of a V slot
   // row maxima of the two half-row warps: [tile][parity][half][row] f32
-  static constexpr int kMaxBytes = kTiles * 4 * kRows * 4;
-  static constexpr int kSmem = kTiles * kQTile + kSlots * kSlot + kMaxBytes + 256;
+  static constexpr int kMaxBytes = kSplit == 2 ? kTiles * 4 * kRows * 4 : 0;
+  static constexpr int kBars = 2 * kSlots + 4 * (kTiles > 1 ? kTiles : 2) + 8;
+  static constexpr int kBarBytes = (kBars * 8 + 8 + 15) / 16 * 16;
+  static constexpr int kSmem = kTiles * kQTile + kSlots * kSlot + kMaxBytes + kBarBytes + 256;
   static constexpr uint32_t kOCol = 0;                 // O_t at t * D
-  static constexpr uint32_t kSCol = kTiles * D;        // two score buffers
-  static_assert(kSCol + 2 * kKeys <= 512, "TMEM columns");
+  static constexpr uint32_t kSCol = kTiles * D;        // score buffers: one a tile, two for one
+  static_assert(kSCol + (kTiles > 1 ? kTiles : 2) * kKeys <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
-  static_assert((2 * kSlots + 8) * 8 + 8 <= 256, "barriers");
 };
 
 struct PkParams {
@@ -112,6 +125,49 @@ __host__ __device__ constexpr uint32_t idesc_bf16_bmn(int M, int N)
   return idesc_bf16(M, N) | (1u << 16);
 }
 
+// The MMA warp runs as a whole, so that the operands' descriptors stay in uniform
+// registers, and one lane of it (`lead`) issues: one lane running the loop alone
+// moves every operand there anew, which made 1200-1700 clocks of a query tile's
+// 500-1000 on the tensor pipe.
+__device__ __forceinline__ uint32_t elect_lane()
+{
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void umma_ss_by(uint32_t lead, uint32_t d, uint64_t a, uint64_t b,
+                                           uint32_t idesc, uint32_t acc)
+{
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_ts_by(uint32_t lead, uint32_t d, uint32_t a_tmem, uint64_t b,
+                                           uint32_t idesc, uint32_t acc)
+{
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_commit_by(uint32_t lead, uint64_t* bar)
+{
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
 // 3-D tiled load, coordinates (x, y, z); x * element size a multiple of 16.
 __device__ __forceinline__ void tma_load_3d(const void* map, uint64_t* bar, void* dst, int x,
                                             int y, int z)
@@ -123,13 +179,13 @@ __device__ __forceinline__ void tma_load_3d(const void* map, uint64_t* bar, void
       : "memory");
 }
 
-// Columns [col0, col0 + D / 2) of one output row from the keys [lo, hi) of its
+// Columns [col0, col0 + N) of one output row from the keys [lo, hi) of its
 // sequence alone (rows key0 + j of k and v), in f32, by one warp.
-template <int D>
+template <int D, int N>
 __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, int kvh, int key0,
                                         int lo, int hi, int col0)
 {
-  constexpr int W = D / 64;                       // dims of a lane
+  constexpr int W = N / 32;                       // dims of a lane
   const int lane = (int)lane_id();
   const __nv_bfloat16* q = p.q + (size_t)row * p.ldq + (size_t)head * D;
   float m = -INFINITY, l = 0.0f, acc[W];
@@ -163,6 +219,80 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
   for (int e = 0; e < W; ++e) o[lane * W + e] = __float2bfloat16_rn(acc[e] / l);
 }
 
+// This thread's N columns of O out of TMEM, scaled, to o (null: nowhere); tells
+// `o_free` once the warp has read it.  Returns whether a NaN was among it.
+template <int N>
+__device__ __forceinline__ bool store_row(uint32_t ocol, bool there, bool sees, float g,
+                                       __nv_bfloat16* o, uint64_t* o_free)
+{
+  bool nan = false;
+#pragma unroll
+  for (int c4 = 0; c4 < N / 32; ++c4) {
+    uint32_t v[32];
+    tmem_ld32(ocol + (uint32_t)(c4 * 32), v);          // whatever it holds, where no key was seen
+    tmem_wait_ld();
+    if (there && c4 + 1 == N / 32) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane_id() == 0) mbar_arrive(o_free);
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float x = sees ? __uint_as_float(v[e]) * g : 0.0f;
+      nan |= x != x;
+      v[e] = __float_as_uint(x);
+    }
+    if (o != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint4 q4;
+        q4.x = pack_bf16(__uint_as_float(v[8 * e + 0]), __uint_as_float(v[8 * e + 1]));
+        q4.y = pack_bf16(__uint_as_float(v[8 * e + 2]), __uint_as_float(v[8 * e + 3]));
+        q4.z = pack_bf16(__uint_as_float(v[8 * e + 4]), __uint_as_float(v[8 * e + 5]));
+        q4.w = pack_bf16(__uint_as_float(v[8 * e + 6]), __uint_as_float(v[8 * e + 7]));
+        *reinterpret_cast<uint4*>(o + c4 * 32 + 8 * e) = q4;
+      }
+    }
+  }
+  return nan;
+}
+
+// One item of work as warp 2 hands it on (head < 0: no more).
+struct PkItem {
+  int head;                       // key/value head
+  int row0, nq, tok0;             // the sequence's rows, the item's first token
+  int key0, nk;                   // the sequence's keys
+  int first, tiles[4];            // first key of the key tiles, their number for each query tile
+};
+
+// Ask for the next CTA of the grid that has not been launched; the 16-byte answer
+// arrives in shared memory and on the barrier.
+__device__ __forceinline__ void ask_next(void* answer, uint64_t* bar)
+{
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
+      "[%1];" ::"r"(smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The answer's blockIdx.x, or -1: none was left.
+__device__ __forceinline__ int next_index(const void* answer)
+{
+  uint32_t x = 0, ok = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "+r"(x), "=r"(ok)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok != 0 ? (int)x : -1;
+}
+
 template <int D>
 __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
     pk_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
@@ -171,7 +301,7 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
                         const __grid_constant__ PkParams p)
 {
   using C = PkCfg<D>;
-  constexpr int T = C::kTiles, R = C::kSlots;
+  constexpr int T = C::kTiles, R = C::kSlots, B = T > 1 ? T : 2, kKeys = C::kKeys;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* s_q = smem_raw;                             // tile t at t * kQTile
   uint8_t* s_ring = s_q + T * C::kQTile;
@@ -179,15 +309,27 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
       reinterpret_cast<float (*)[2][2][kRows]>(s_ring + R * C::kSlot);
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_ring + R * C::kSlot + C::kMaxBytes);
   uint64_t* q_full = bars;
-  uint64_t* full = q_full + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* full = q_empty + 1;
   uint64_t* empty = full + R;
   uint64_t* s_full = empty + R;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_done = p_full + 2;
-  uint64_t* drain = o_done + 2;
+  uint64_t* p_full = s_full + B;
+  uint64_t* o_done = p_full + B;
+  uint64_t* o_free = o_done + B;
+  uint64_t* item_full = o_free + B;
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* asked = item_empty + 2;
+  uint64_t* drain = asked + 1;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  const int warp = threadIdx.x >> 5;
+  uint8_t* tail = s_ring + R * C::kSlot + C::kMaxBytes + C::kBarBytes;
+  uint8_t* s_answer = tail;                            // 16 bytes
+  volatile int* s_fail = reinterpret_cast<volatile int*>(tail + 16);    // one a query tile
+  PkItem* s_item = reinterpret_cast<PkItem*>(tail + 32);                // two
+  static_assert(32 + 2 * sizeof(PkItem) <= 256, "tail");
+
+  // the same for all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const uint32_t lane = threadIdx.x & 31;
   if ((smem_u32(smem_raw) & 1023u) != 0) {             // the swizzle's atom
     if (threadIdx.x == 0) atomicCAS(p.err, 0, PERR_DRAIN);
@@ -196,15 +338,23 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < R; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < B; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&p_full[i], C::kGroup);
       mbar_init(&o_done[i], 1);
+      mbar_init(&o_free[i], C::kGroup);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 2 + C::kGroup * T);
+      s_fail[i] = 0;
+    }
+    mbar_init(asked, 1);
     mbar_init(drain, 1);
     *s_abort = 0;
     fence_mbar_init();
@@ -225,332 +375,439 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // the CTA's sequence, tokens and keys.  Slots run backwards, so that a
-  // causal sequence's longest tiles start first.
-  const int kvh = (int)(blockIdx.x % (unsigned)p.kv_heads);
-  const int slots = slot_count(p.rows, p.seqs, T * p.tq, 1);
-  const int slot = slots - 1 - (int)(blockIdx.x / (unsigned)p.kv_heads);
-  const int seq = find_seq(p.cu_q, p.seqs, p.rows, T * p.tq, 1, slot);
-  const int row0 = clamp_int(p.cu_q[seq], 0, p.rows);
-  const int nq = clamp_int(p.cu_q[seq + 1], row0, p.rows) - row0;
-  const int key0 = clamp_int(p.cu_k[seq], 0, p.keys);
-  const int nk = clamp_int(p.cu_k[seq + 1], key0, p.keys) - key0;
-  const int tok0 = max(0, slot - slot_base(row0, seq, T * p.tq, 1)) * (T * p.tq);
-  // keys any of the rows sees: from the first row's low to the last one's high
-  const int shift = nk - nq;
-  const int jb = key_low(shift + tok0, p.window);
-  int n_t[2] = {0, 0};                                 // key tiles of each query tile
+  // Items pass through two places in turn; each role counts them (`it`) and what
+  // it has waited for and signalled since the CTA began, so that the barriers'
+  // phases run on from item to item.
+  if (warp == 2) {
+    // ------------------------------------------------------------ items
+    const int slots = slot_count(p.rows, p.seqs, T * p.tq, 1);
+    int index = (int)blockIdx.x;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      // the answer is read before the next question goes out to its place
+      if (index >= 0 && lane == 0) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        ask_next(s_answer, asked);
+      }
+      PkItem w;
+      w.head = -1;
+      if (index >= 0) {
+        // slots run backwards, so that a causal sequence's longest items are first
+        w.head = (int)((unsigned)index % (unsigned)p.kv_heads);
+        const int slot = slots - 1 - (int)((unsigned)index / (unsigned)p.kv_heads);
+        const int seq = find_seq(p.cu_q, p.seqs, p.rows, T * p.tq, 1, slot);
+        w.row0 = clamp_int(p.cu_q[seq], 0, p.rows);
+        w.nq = clamp_int(p.cu_q[seq + 1], w.row0, p.rows) - w.row0;
+        w.key0 = clamp_int(p.cu_k[seq], 0, p.keys);
+        w.nk = clamp_int(p.cu_k[seq + 1], w.key0, p.keys) - w.key0;
+        w.tok0 = max(0, slot - slot_base(w.row0, seq, T * p.tq, 1)) * (T * p.tq);
+        // keys any of the rows sees: from the first row's low to the last one's high
+        const int shift = w.nk - w.nq;
+        w.first = key_low(shift + w.tok0, p.window);
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int a = tok0 + t * p.tq, b = min(a + p.tq, nq);
-    if (b > a) {
-      const int je = key_high(shift + b - 1, nk, p.causal);
-      n_t[t] = je > jb ? (je - jb + kKeys - 1) / kKeys : 0;
-    }
-  }
-  const int n = max(n_t[0], n_t[1]);
-
-  if (warp == 0) {
-    // ------------------------------------------------------------- TMA
-    if (lane == 0 && n > 0) {
-      uint32_t armed = 0, armed_par = 0;
-      const int boxes = C::kTiles * (D / 64);
-      mbar_arrive_expect_tx(q_full, (uint32_t)(boxes * p.group * p.tq * 128));
-      for (int t = 0; t < T; ++t)
-        for (int a = 0; a < D / 64; ++a)
-          tma_load_3d(&tm_q, q_full, s_q + t * C::kQTile + a * C::kAtom, a * 64,
-                      kvh * p.group, row0 + tok0 + t * p.tq);
-      int used = 0;
-      bool ok = true;
-      // one slot: `v` selects V, part its half at width 256
-      auto load = [&](bool v, int j) {
-        for (int part = 0; ok && part < C::kParts; ++part, ++used) {
-          const int st = used % R;
-          const uint32_t ph = (uint32_t)(used / R) & 1u;
-          ok = mbar_wait(&empty[st], ph ^ 1u, s_abort, p.err, PERR_PRODUCER);
-          if (!ok) break;
-          uint8_t* dst = s_ring + st * C::kSlot;
-          const int key = key0 + jb + j * kKeys;
-          mbar_arrive_expect_tx(&full[st], C::kSlot);
-          if (v) {
-            for (int a = 0; a < D / 64; ++a)
-              tma_load_3d(&tm_v, &full[st], dst + a * C::kVKeys * 128, a * 64, kvh,
-                          key + part * C::kVKeys);
-          } else {
-            constexpr int A = D / 64 / C::kParts;
-            for (int a = 0; a < A; ++a)
-              tma_load_3d(&tm_k, &full[st], dst + a * C::kAtom, (part * A + a) * 64, kvh, key);
+        for (int t = 0; t < 4; ++t) w.tiles[t] = 0;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const int a = w.tok0 + t * p.tq, b = min(a + p.tq, w.nq);
+          if (b > a) {
+            const int end = key_high(shift + b - 1, w.nk, p.causal);
+            w.tiles[t] = end > w.first ? (end - w.first + kKeys - 1) / kKeys : 0;
           }
-          armed |= 1u << st;
-          armed_par = (armed_par & ~(1u << st)) | (ph << st);
         }
-      };
-      load(false, 0);
-      for (int j = 0; ok && j < n; ++j) {
-        if (T == 1 && j + 1 < n) load(false, j + 1);
-        load(true, j);
-        if (T == 2 && j + 1 < n) load(false, j + 1);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u,
+                                             s_abort, p.err, PERR_ITEM));
+      if (ok && lane == 0) {
+        s_item[it & 1] = w;
+        mbar_arrive(&item_full[it & 1]);
+      }
+      if (index < 0) break;
+      // every question is waited for, so that no answer is under way at the end
+      volatile int no_abort = 0;
+      const bool told = __all_sync(
+          0xffffffffu, mbar_wait(asked, (uint32_t)it & 1u, &no_abort, p.err, PERR_DRAIN));
+      ok = ok && told;
+      if (ok) index = next_index(s_answer);
+      __syncwarp();
+    }
+  } else if (warp == 0) {
+    // ------------------------------------------------------------- TMA
+    if (lane == 0) {
+      uint32_t armed = 0, armed_par = 0, q_armed = 0;
+      int used = 0, with_keys = 0;                     // ring slots, items that have keys
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        ok = mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_abort, p.err, PERR_PRODUCER);
+        if (!ok) break;
+        const PkItem w = s_item[it & 1];
+        mbar_arrive(&item_empty[it & 1]);
+        if (w.head < 0) break;
+        const int n = max(max(w.tiles[0], w.tiles[1]), max(w.tiles[2], w.tiles[3]));
+        if (n == 0) continue;
+        // Q's place is free once the item before has its last scores
+        ok = mbar_wait(q_empty, ((uint32_t)with_keys & 1u) ^ 1u, s_abort, p.err, PERR_PRODUCER);
+        if (!ok) break;
+        mbar_arrive_expect_tx(q_full, (uint32_t)(T * (D / 64) * p.group * p.tq * 128));
+        for (int t = 0; t < T; ++t)
+          for (int a = 0; a < D / 64; ++a)
+            tma_load_3d(&tm_q, q_full, s_q + t * C::kQTile + a * C::kQAtom, a * 64,
+                        w.head * p.group, w.row0 + w.tok0 + t * p.tq);
+        ++with_keys;
+        q_armed = 1;
+        // one slot: `v` selects V, part its half at width 256
+        auto load = [&](bool v, int j) {
+          for (int part = 0; ok && part < C::kParts; ++part, ++used) {
+            const int st = used % R;
+            const uint32_t ph = (uint32_t)(used / R) & 1u;
+            ok = mbar_wait(&empty[st], ph ^ 1u, s_abort, p.err, PERR_PRODUCER);
+            if (!ok) break;
+            uint8_t* dst = s_ring + st * C::kSlot;
+            const int key = w.key0 + w.first + j * kKeys;
+            mbar_arrive_expect_tx(&full[st], C::kSlot);
+            if (v) {
+              for (int a = 0; a < D / 64; ++a)
+                tma_load_3d(&tm_v, &full[st], dst + a * C::kVKeys * 128, a * 64, w.head,
+                            key + part * C::kVKeys);
+            } else {
+              constexpr int A = D / 64 / C::kParts;
+              for (int a = 0; a < A; ++a)
+                tma_load_3d(&tm_k, &full[st], dst + a * C::kKAtom, (part * A + a) * 64, w.head,
+                            key);
+            }
+            armed |= 1u << st;
+            armed_par = (armed_par & ~(1u << st)) | (ph << st);
+          }
+        };
+        load(false, 0);
+        for (int j = 0; ok && j < n; ++j) {
+          if (T == 1 && j + 1 < n) load(false, j + 1);
+          load(true, j);
+          if (T > 1 && j + 1 < n) load(false, j + 1);
+        }
       }
       // Every load lands before the CTA may exit.
       volatile int no_abort = 0;
-      mbar_wait(q_full, 0, &no_abort, p.err, PERR_DRAIN);
+      if (q_armed)
+        mbar_wait(q_full, (uint32_t)(with_keys - 1) & 1u, &no_abort, p.err, PERR_DRAIN);
       for (int st = 0; st < R; ++st)
         if (armed & (1u << st))
           mbar_wait(&full[st], (armed_par >> st) & 1u, &no_abort, p.err, PERR_DRAIN);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t idesc_s = idesc_bf16(kRows, kKeys);
-      constexpr uint32_t idesc_o = idesc_bf16_bmn(kRows, D);
-      int used = 0;                                    // ring slots taken so far
-      auto wait_slots = [&](int at) {
-        for (int part = 0; part < C::kParts; ++part) {
-          const int u = at + part;
-          if (!mbar_wait(&full[u % R], (uint32_t)(u / R) & 1u, s_abort, p.err, PERR_MMA))
-            return false;
-        }
+    constexpr uint32_t idesc_s = idesc_bf16(kRows, kKeys);
+    constexpr uint32_t idesc_o = idesc_bf16_bmn(kRows, D);
+    const uint32_t lead = elect_lane();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, s_abort, p.err, PERR_MMA)) != 0;
+    };
+    // a ring of slots: the next one and the parity of its round
+    uint32_t slot = 0, round = 0;
+    auto next_slot = [&]() {
+      if (++slot == (uint32_t)R) {
+        slot = 0;
+        round ^= 1u;
+      }
+    };
+    const uint64_t q_desc = sdesc_k128_sw128(smem_u32(s_q));
+    const uint64_t k_desc = sdesc_k128_sw128(smem_u32(s_ring));
+    const uint64_t v_desc = sdesc_mn_sw128(smem_u32(s_ring), C::kVKeys * 128);
+    // scores for query tile t into buffer b of the k steps that key slot `at`
+    // holds (part: its half at width 256)
+    auto issue_s = [&](int t, uint32_t b, uint32_t at, int part) {
+      constexpr int A = D / 64 / C::kParts;            // 64-dim atoms of a slot
+      const uint32_t d = tm + C::kSCol + b * (uint32_t)kKeys;
+      const uint64_t qd = q_desc + (uint64_t)(((t * C::kQTile + part * A * C::kQAtom) >> 4));
+      const uint64_t kd = k_desc + (uint64_t)(at * (uint32_t)(C::kSlot >> 4));
+#pragma unroll
+      for (int kk = 0; kk < A * 4; ++kk)
+        umma_ss_by(lead, d, qd + (uint64_t)((kk >> 2) * (C::kQAtom >> 4) + 2 * (kk & 3)),
+                   kd + (uint64_t)((kk >> 2) * (C::kKAtom >> 4) + 2 * (kk & 3)), idesc_s,
+                   part > 0 || kk > 0 ? 1u : 0u);
+    };
+    // O += P V over the keys of value slot `at`
+    auto issue_pv = [&](int t, uint32_t b, uint32_t at, int part, bool first) {
+      const uint32_t pa = tm + C::kSCol + b * (uint32_t)kKeys + (uint32_t)(part * C::kVKeys / 2);
+      const uint64_t vd = v_desc + (uint64_t)(at * (uint32_t)(C::kSlot >> 4));
+#pragma unroll
+      for (int kk = 0; kk < C::kVKeys / 16; ++kk)
+        umma_ts_by(lead, tm + C::kOCol + (uint32_t)(t * D), pa + (uint32_t)(kk * 8),
+                   vd + (uint64_t)(kk * (16 * 128 >> 4)), idesc_o,
+                   !first || part > 0 || kk > 0 ? 1u : 0u);
+    };
+    uint32_t with_keys = 0;                            // items that have keys
+    uint32_t step[T] = {}, opened[T] = {};             // score tiles and items, a query tile
+    bool ok = true;
+    for (uint32_t it = 0; ok; ++it) {
+      ok = wait(&item_full[it & 1], (it >> 1) & 1u);
+      if (!ok) break;
+      const PkItem* w = &s_item[it & 1];
+      const int head = __shfl_sync(0xffffffffu, w->head, 0);
+      int tiles[T], n = 0;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        tiles[t] = __shfl_sync(0xffffffffu, w->tiles[t], 0);
+        n = max(n, tiles[t]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+      if (head < 0) break;
+      if (n == 0) continue;
+      ok = wait(q_full, with_keys & 1u);
+      if (!ok) break;
+      ++with_keys;
+      if constexpr (T > 1) {
+        ok = wait(&full[slot], round);
+        if (!ok) break;
         tc_fence_after();
-        return true;
-      };
-      auto free_slots = [&](int at) {
-        for (int part = 0; part < C::kParts; ++part) umma_commit(&empty[(at + part) % R]);
-      };
-      // scores of key tile in slot(s) `at` for query tile t into buffer b
-      auto issue_s = [&](int t, int b, int at) {
-        const uint32_t sq = smem_u32(s_q + t * C::kQTile);
-        const uint32_t d = tmem + C::kSCol + (uint32_t)b * kKeys;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          constexpr int A = D / 64 / C::kParts;        // 64-dim atoms of a slot
-          const int a = kk >> 2;
-          const uint32_t sk = smem_u32(s_ring + ((at + a / A) % R) * C::kSlot) +
-                              (uint32_t)((a % A) * C::kAtom);
-          umma_f16_ss(d, sdesc_k128_sw128(sq + (uint32_t)(a * C::kAtom)) + (uint64_t)(2 * (kk & 3)),
-                      sdesc_k128_sw128(sk) + (uint64_t)(2 * (kk & 3)), idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[b]);
-      };
-      auto issue_pv = [&](int t, int b, int at, bool first) {
-        const uint32_t pa = tmem + C::kSCol + (uint32_t)b * kKeys;
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk) {
-          constexpr int KS = C::kVKeys / 16;           // k steps of a slot
-          const uint32_t sv = smem_u32(s_ring + ((at + kk / KS) % R) * C::kSlot) +
-                              (uint32_t)((kk % KS) * 16 * 128);
-          umma_f16_ts(tmem + C::kOCol + (uint32_t)(t * D), pa + (uint32_t)(kk * 8),
-                      sdesc_mn_sw128(sv, C::kVKeys * 128), idesc_o, !first || kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&o_done[t]);
-      };
-      bool ok = mbar_wait(q_full, 0, s_abort, p.err, PERR_MMA) && wait_slots(0);
-      if (T == 2) {
-        if (ok) {
-          for (int t = 0; t < T; ++t)
-            if (n_t[t] > 0) issue_s(t, t, 0);
-          free_slots(0);
-        }
-        used = C::kParts;
+        for (int t = 0; t < T; ++t)
+          if (tiles[t] > 0) {
+            issue_s(t, (uint32_t)t, slot, 0);
+            umma_commit_by(lead, &s_full[t]);
+          }
+        umma_commit_by(lead, &empty[slot]);
+        if (n == 1) umma_commit_by(lead, q_empty);
+        next_slot();
         for (int j = 0; ok && j < n; ++j) {
-          const int av = used, ak = used + C::kParts;  // V_j, K_{j+1}
+          const uint32_t av = slot, av_round = round;  // V_j, then K_{j+1}
+          next_slot();
+          const uint32_t ak = slot, ak_round = round;
           const bool more = j + 1 < n;
           bool have_v = false, have_k = false;
-          for (int t = 0; ok && t < T; ++t) {
-            if (j >= n_t[t]) continue;
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            if (!ok || j >= tiles[t]) continue;
             // P V, then the tile's next S (in order: the S MMA overwrites the
-            // buffer only after this P V has read P from it)
-            ok = mbar_wait(&p_full[t], (uint32_t)j & 1u, s_abort, p.err, PERR_MMA) &&
-                 (have_v || wait_slots(av));
-            if (!ok) break;
+            // buffer only after this P V has read P from it); an item's first P V
+            // overwrites O, which the softmax must have read
+            ok = wait(&p_full[t], step[t] & 1u);
+            ++step[t];
+            if (ok && j == 0) ok = wait(&o_free[t], (opened[t]++ & 1u) ^ 1u);
+            if (ok && !have_v) ok = wait(&full[av], av_round);
             have_v = true;
+            if (!ok) continue;
             tc_fence_after();
-            issue_pv(t, t, av, j == 0);
-            if (j + 1 < n_t[t]) {
-              ok = have_k || wait_slots(ak);
-              if (!ok) break;
+            issue_pv(t, (uint32_t)t, av, 0, j == 0);
+            umma_commit_by(lead, &o_done[t]);
+            if (j + 1 < tiles[t]) {
+              if (!have_k) ok = wait(&full[ak], ak_round);
               have_k = true;
-              issue_s(t, t, ak);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_s(t, (uint32_t)t, ak, 0);
+              umma_commit_by(lead, &s_full[t]);
             }
           }
           if (!ok) break;
-          free_slots(av);
-          if (more) free_slots(ak);
-          used = ak + (more ? C::kParts : 0);
+          umma_commit_by(lead, &empty[av]);
+          if (more) {
+            umma_commit_by(lead, &empty[ak]);
+            next_slot();
+          }
+          if (j + 2 == n) umma_commit_by(lead, q_empty);
         }
       } else {
-        int ak[2] = {0, 0}, av = 0;
-        if (ok) {
-          issue_s(0, 0, 0);
-          free_slots(0);
-        }
-        used = C::kParts;
-        for (int j = 0; ok && j < n; ++j) {
+        // S_0, then S_{j+1} and P_j V_j by turns
+        const uint32_t base = step[0];
+        for (int j = -1; ok && j < n; ++j) {
           if (j + 1 < n) {
-            ak[0] = used;
-            used += C::kParts;
-            ok = wait_slots(ak[0]);
+            const uint32_t b = (base + (uint32_t)(j + 1)) & 1u;
+#pragma unroll
+            for (int part = 0; part < C::kParts; ++part) {
+              if (ok) ok = wait(&full[slot], round);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_s(0, b, slot, part);
+              umma_commit_by(lead, &empty[slot]);
+              next_slot();
+            }
             if (!ok) break;
-            issue_s(0, (j + 1) & 1, ak[0]);
-            free_slots(ak[0]);
+            umma_commit_by(lead, &s_full[b]);
+            if (j + 2 == n) umma_commit_by(lead, q_empty);
           }
-          av = used;
-          used += C::kParts;
-          ok = mbar_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1u, s_abort, p.err, PERR_MMA) &&
-               wait_slots(av);
+          if (j < 0) continue;
+          const uint32_t at = base + (uint32_t)j;
+          ok = wait(&p_full[at & 1u], (at >> 1) & 1u);
+          if (ok && j == 0) ok = wait(&o_free[0], (opened[0]++ & 1u) ^ 1u);
+#pragma unroll
+          for (int part = 0; part < C::kParts; ++part) {
+            if (ok) ok = wait(&full[slot], round);
+            if (!ok) continue;
+            tc_fence_after();
+            issue_pv(0, at & 1u, slot, part, j == 0);
+            umma_commit_by(lead, &empty[slot]);
+            next_slot();
+          }
           if (!ok) break;
-          issue_pv(0, j & 1, av, j == 0);
-          free_slots(av);
+          umma_commit_by(lead, &o_done[0]);
         }
+        step[0] = base + (uint32_t)n;
       }
-      umma_commit(drain);
-      volatile int no_abort = 0;
-      mbar_wait(drain, 0, &no_abort, p.err, PERR_DRAIN);
     }
+    umma_commit_by(lead, drain);
+    volatile int no_abort = 0;
+    mbar_wait(drain, 0, &no_abort, p.err, PERR_DRAIN);
+    __syncwarp();
   } else if (warp >= 4) {
     // ---------------------------------------------------------- softmax
-    // Within a tile the first four warps take score columns [0, 64), the next
-    // four [64, 128) of the same rows.
-    const int t = (warp - 4) >> 3;
-    const int hh = ((warp - 4) >> 2) & 1;
+    // Four warps a tile with a row a thread, or eight: the first four take score
+    // columns [0, 64), the next four [64, 128) of the same rows.
+    constexpr int kSplit = C::kSplit;
+    const int t = (warp - 4) / C::kGroup;
+    const int hh = ((warp - 4) >> 2) & (kSplit - 1);
     const int r = (warp & 3) * 32 + (int)lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ocol = tmem + lane_base + C::kOCol + (uint32_t)(t * D + hh * (D / 2));
+    const uint32_t ocol = tmem + lane_base + C::kOCol + (uint32_t)(t * D + hh * (D / kSplit));
     const float c = p.c;
-    const int nt = n_t[t];
-    // this thread's row: token and head, and the keys it sees
-    const int tok = tok0 + t * p.tq + r / p.group;
-    const bool valid_row = r < p.tq * p.group && tok < nq;
-    const int lo = key_low(shift + tok, p.window);
-    const int hi = valid_row ? key_high(shift + tok, nk, p.causal) : 0;
-    // key tiles that every valid row of this query tile sees whole
-    const int a_tok = tok0 + t * p.tq, b_tok = min(a_tok + p.tq, nq) - 1;
-    const int all_lo = key_low(shift + b_tok, p.window);
-    const int all_hi = key_high(shift + a_tok, nk, p.causal);
-    float m_run = -INFINITY, l_run = 0.0f;
+    uint32_t step = 0, swap = 0;                       // score tiles, exchanges so far
     bool ok = true;
-    // Every warp of a tile takes the same nt + 1 named barriers, also after an
-    // abort (which then only skips the TMEM work), so none is left waiting.
-    for (int i = 0; i < nt; ++i) {
-      const int sb = T == 2 ? t : (i & 1);
-      const uint32_t ph = T == 2 ? (uint32_t)i & 1u : (uint32_t)(i >> 1) & 1u;
-      const uint32_t scol = tmem + lane_base + C::kSCol + (uint32_t)(sb * kKeys);
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&s_full[sb], ph, s_abort, p.err, PERR_SOFTMAX));
-      uint32_t a[32], b[32];
-      tc_fence_after();
-      tmem_ld32(scol + (uint32_t)(hh * 64), a);
-      tmem_ld32(scol + (uint32_t)(hh * 64 + 32), b);
-      tmem_wait_ld();
-      const int j0 = jb + i * kKeys;
-      if (j0 < all_lo || j0 + kKeys > all_hi) {
-        const int from = lo - j0 - hh * 64, to = hi - j0 - hh * 64;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          if (e < from || e >= to) a[e] = 0xff800000u;             // -inf
-          if (32 + e < from || 32 + e >= to) b[e] = 0xff800000u;
-        }
+#pragma unroll 1
+    for (int it = 0;; ++it) {
+      // Two warps a row meet at barriers, so all warps of a tile agree on going on:
+      // a wait that failed is told before one, and their number in an item is the
+      // same for all.
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u,
+                                                   s_abort, p.err, PERR_SOFTMAX));
+      if (kSplit == 1) {
+        if (!ok) break;
+      } else {
+        if (!ok && lane == 0) s_fail[t] = 1;
+        named_bar_sync(1 + t, 256);
+        if (s_fail[t] != 0) break;
       }
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        m4[0] = max3f(m4[0], __uint_as_float(a[e]), __uint_as_float(a[e + 1]));
-        m4[1] = max3f(m4[1], __uint_as_float(a[e + 2]), __uint_as_float(a[e + 3]));
-        m4[2] = max3f(m4[2], __uint_as_float(b[e]), __uint_as_float(b[e + 1]));
-        m4[3] = max3f(m4[3], __uint_as_float(b[e + 2]), __uint_as_float(b[e + 3]));
+      // the item stays in its place until this role is through with it
+      const PkItem* w = &s_item[it & 1];
+      if (w->head < 0) break;
+      const int nt = w->tiles[t];
+      int j0 = w->first;
+      // the keys this thread's row sees, and those that all valid rows of the
+      // query tile see
+      int lo, hi, all_lo, all_hi;
+      {
+        const int tok = w->tok0 + t * p.tq + r / p.group, shift = w->nk - w->nq;
+        const bool valid_row = r < p.tq * p.group && tok < w->nq;
+        lo = key_low(shift + tok, p.window);
+        hi = valid_row ? key_high(shift + tok, w->nk, p.causal) : 0;
+        const int a_tok = w->tok0 + t * p.tq, b_tok = min(a_tok + p.tq, w->nq) - 1;
+        all_lo = key_low(shift + b_tok, p.window);
+        all_hi = key_high(shift + a_tok, w->nk, p.causal);
       }
-      // the row's max over both halves: exchange through shared memory (both
-      // halves have their scores in registers after this barrier, so either
-      // may then overwrite the TMEM columns with P)
-      s_mx[t][i & 1][hh][r] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      named_bar_sync(1 + t, 256);
-      if (!ok) continue;
-      const float m_tile = fmaxf(s_mx[t][i & 1][0][r], s_mx[t][i & 1][1][r]) * c;
-      // a row's first visible tile sets its maximum; later it moves only when
-      // it grows by more than 2^kGrow (until then P stays below 2^kGrow)
-      const bool need = m_tile > m_run + kGrow;
-      const bool rescale = i > 0 && __any_sync(0xffffffffu, need);
-      float f = 1.0f;
-      if (need) {
-        f = fast_exp2(m_run - m_tile);
-        l_run *= f;
-        m_run = m_tile;
-      }
-      const float nm = m_run == -INFINITY ? 0.0f : -m_run;
-      const unsigned long long c2 = pair2(__float_as_uint(c), __float_as_uint(c));
-      const unsigned long long nm2 = pair2(__float_as_uint(nm), __float_as_uint(nm));
-      unsigned long long sa = 0ull, sb2 = 0ull;
-      uint32_t pk[32];
-      fa3_exp(a, b, c2, nm2, pk, sa, sb2);
-      tmem_st32(scol + (uint32_t)(hh * 32), pk);
-      const unsigned long long st2 = fadd2(sa, sb2);
-      l_run += __uint_as_float((uint32_t)st2) + __uint_as_float((uint32_t)(st2 >> 32));
-      if (rescale)
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (uint32_t)(i - 1) & 1u, s_abort, p.err,
-                                               PERR_SOFTMAX));
-      if (rescale && ok) {
+      float m_run = -INFINITY, l_run = 0.0f;
+#pragma unroll 1
+      for (int i = 0; i < nt; ++i, ++step, ++swap, j0 += kKeys) {
+        const int sb = T > 1 ? t : (int)(step & 1u);
+        const uint32_t ph = T > 1 ? step & 1u : (step >> 1) & 1u;
+        const uint32_t scol = tmem + lane_base + C::kSCol + (uint32_t)(sb * kKeys);
+        ok = __all_sync(0xffffffffu,
+                        ok && mbar_wait(&s_full[sb], ph, s_abort, p.err, PERR_SOFTMAX));
+        uint32_t a[32], b[32];
         tc_fence_after();
+        tmem_ld32(scol + (uint32_t)(hh * 64), a);
+        tmem_ld32(scol + (uint32_t)(hh * 64 + 32), b);
+        tmem_wait_ld();
+        if (j0 < all_lo || j0 + kKeys > all_hi) {
+          const int from = lo - j0 - hh * 64, to = hi - j0 - hh * 64;
 #pragma unroll
-        for (int c4 = 0; c4 < D / 64; ++c4) {
-          uint32_t v[32];
-          tmem_ld32(ocol + (uint32_t)(c4 * 32), v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-          tmem_st32(ocol + (uint32_t)(c4 * 32), v);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (ok && lane == 0) mbar_arrive(&p_full[sb]);
-    }
-    // the row's sum over both halves (parity slot nt & 1 is free now)
-    s_mx[t][nt & 1][hh][r] = l_run;
-    named_bar_sync(1 + t, 256);
-    const float l_row = s_mx[t][nt & 1][0][r] + s_mx[t][nt & 1][1][r];
-    if (ok && nt > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (uint32_t)(nt - 1) & 1u, s_abort, p.err,
-                                             PERR_SOFTMAX));
-    if (ok) {
-      tc_fence_after();
-      const bool sees = hi > lo;
-      const int row = row0 + tok;
-      const int head = kvh * p.group + r % p.group;
-      const float g = 1.0f / l_row;
-      __nv_bfloat16* orow = p.o + (size_t)row * p.ldo + (size_t)head * D + hh * (D / 2);
-      bool nan = false;
-#pragma unroll
-      for (int c4 = 0; c4 < D / 64; ++c4) {
-        uint32_t v[32];
-        if (nt > 0) {
-          tmem_ld32(ocol + (uint32_t)(c4 * 32), v);
-          tmem_wait_ld();
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = nt > 0 && sees ? __uint_as_float(v[e]) * g : 0.0f;
-          nan |= x != x;
-          v[e] = __float_as_uint(x);
-        }
-        if (valid_row) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 w;
-            w.x = pack_bf16(__uint_as_float(v[8 * e + 0]), __uint_as_float(v[8 * e + 1]));
-            w.y = pack_bf16(__uint_as_float(v[8 * e + 2]), __uint_as_float(v[8 * e + 3]));
-            w.z = pack_bf16(__uint_as_float(v[8 * e + 4]), __uint_as_float(v[8 * e + 5]));
-            w.w = pack_bf16(__uint_as_float(v[8 * e + 6]), __uint_as_float(v[8 * e + 7]));
-            *reinterpret_cast<uint4*>(orow + c4 * 32 + 8 * e) = w;
+          for (int e = 0; e < 32; ++e) {
+            if (e < from || e >= to) a[e] = 0xff800000u;             // -inf
+            if (32 + e < from || 32 + e >= to) b[e] = 0xff800000u;
           }
         }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          m4[0] = max3f(m4[0], __uint_as_float(a[e]), __uint_as_float(a[e + 1]));
+          m4[1] = max3f(m4[1], __uint_as_float(a[e + 2]), __uint_as_float(a[e + 3]));
+          m4[2] = max3f(m4[2], __uint_as_float(b[e]), __uint_as_float(b[e + 1]));
+          m4[3] = max3f(m4[3], __uint_as_float(b[e + 2]), __uint_as_float(b[e + 3]));
+        }
+        // the row's max over both halves: exchange through shared memory (both
+        // halves have their scores in registers after this barrier, so either
+        // may then overwrite the TMEM columns with P)
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if (kSplit == 2) {
+          s_mx[t][swap & 1u][hh][r] = mx;
+          named_bar_sync(1 + t, 256);
+          mx = fmaxf(s_mx[t][swap & 1u][0][r], s_mx[t][swap & 1u][1][r]);
+        }
+        if (!ok) continue;
+        const float m_tile = mx * c;
+        // a row's first visible tile sets its maximum; later it moves only when
+        // it grows by more than 2^kGrow (until then P stays below 2^kGrow)
+        const bool need = m_tile > m_run + kGrow;
+        const bool rescale = i > 0 && __any_sync(0xffffffffu, need);
+        float f = 1.0f;
+        if (need) {
+          f = fast_exp2(m_run - m_tile);
+          l_run *= f;
+          m_run = m_tile;
+        }
+        const float nm = m_run == -INFINITY ? 0.0f : -m_run;
+        const unsigned long long c2 = pair2(__float_as_uint(c), __float_as_uint(c));
+        const unsigned long long nm2 = pair2(__float_as_uint(nm), __float_as_uint(nm));
+        unsigned long long sa = 0ull, sb2 = 0ull;
+        uint32_t pk[32];
+        fa3_exp(a, b, c2, nm2, pk, sa, sb2);
+        tmem_st32(scol + (uint32_t)(hh * 32), pk);
+        const unsigned long long st2 = fadd2(sa, sb2);
+        l_run += __uint_as_float((uint32_t)st2) + __uint_as_float((uint32_t)(st2 >> 32));
+        if (rescale)
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&o_done[t], (step - 1u) & 1u, s_abort, p.err, PERR_SOFTMAX));
+        if (rescale && ok) {
+          tc_fence_after();
+#pragma unroll
+          for (int c4 = 0; c4 < D / kSplit / 32; ++c4) {
+            uint32_t v[32];
+            tmem_ld32(ocol + (uint32_t)(c4 * 32), v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+            tmem_st32(ocol + (uint32_t)(c4 * 32), v);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&p_full[sb]);
       }
+      // the row's sum over both halves
+      float l_row = l_run;
+      if (kSplit == 2) {
+        s_mx[t][swap & 1u][hh][r] = l_run;
+        named_bar_sync(1 + t, 256);
+        l_row = s_mx[t][swap & 1u][0][r] + s_mx[t][swap & 1u][1][r];
+        ++swap;
+      }
+      // A wait on a parity must not be two phases ahead.  With several tiles the last
+      // scores followed the last P V but one; with one tile they ran before it.
+      if (T == 1 && ok && nt > 1)
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&o_done[t], (step - 2u) & 1u, s_abort, p.err, PERR_SOFTMAX));
+      if (ok && nt > 0)
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&o_done[t], (step - 1u) & 1u, s_abort, p.err, PERR_SOFTMAX));
+      if (!ok) continue;
+      tc_fence_after();
+      const bool sees = nt > 0 && hi > lo;
+      const int tok = w->tok0 + t * p.tq + r / p.group;
+      const bool valid_row = r < p.tq * p.group && tok < w->nq;
+      const int row = w->row0 + tok, head = w->head * p.group + r % p.group;
+      const float g = 1.0f / l_row;
+      __nv_bfloat16* orow = p.o + (size_t)row * p.ldo + (size_t)head * D + hh * (D / kSplit);
+      const bool nan = store_row<D / kSplit>(ocol, nt > 0, sees, g, valid_row ? orow : nullptr, &o_free[t]);
       uint32_t bad = __ballot_sync(0xffffffffu, nan && valid_row);
       while (bad != 0) {
         const int src = __ffs((int)bad) - 1;
         bad &= bad - 1;
-        repair_row<D>(p, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src),
-                      kvh, key0, __shfl_sync(0xffffffffu, lo, src),
-                      __shfl_sync(0xffffffffu, hi, src), hh * (D / 2));
+        repair_row<D, D / kSplit>(p, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src),
+                      w->head, w->key0, __shfl_sync(0xffffffffu, lo, src),
+                      __shfl_sync(0xffffffffu, hi, src), hh * (D / kSplit));
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[it & 1]);
     }
   }
   tc_fence_before();
@@ -615,7 +872,7 @@ int pk_launch(const PackedAttention& a, int* err, cudaStream_t s)
   // no keys at all: every row is empty and nothing loads through mk and mv
   const bool none = a.keys == 0;
   if (!pk_encode(&mq, a.q, D, a.heads, a.rows, a.ldq, p.group, p.tq) ||
-      !pk_encode(&mk, none ? a.q : a.k, D, a.kv_heads, none ? 1 : a.keys, a.ldk, 1, kKeys) ||
+      !pk_encode(&mk, none ? a.q : a.k, D, a.kv_heads, none ? 1 : a.keys, a.ldk, 1, C::kKeys) ||
       !pk_encode(&mv, none ? a.q : a.v, D, a.kv_heads, none ? 1 : a.keys, a.ldv, 1, C::kVKeys))
     return -1;
   const long long grid =
