@@ -219,39 +219,68 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
   for (int e = 0; e < W; ++e) o[lane * W + e] = __float2bfloat16_rn(acc[e] / l);
 }
 
-// This thread's N columns of O out of TMEM, scaled, to o (null: nowhere); tells
-// `o_free` once the warp has read it.  Returns whether a NaN was among it.
+// Bits [from, to) of 32, both bounds anywhere.
+__device__ __forceinline__ uint32_t bits_from_to(int from, int to)
+{
+  const uint32_t below = to >= 32 ? 0xffffffffu : to <= 0 ? 0u : (1u << to) - 1u;
+  const uint32_t skip = from >= 32 ? 0xffffffffu : from <= 0 ? 0u : (1u << from) - 1u;
+  return below & ~skip;
+}
+
+// N columns of this thread's row of O out of TMEM, scaled, to o + at (at < 0:
+// nowhere); tells `o_free` once the warp has read it.  Returns whether a NaN was
+// among it.  Eight lanes exchange their rows' 16-byte pieces so that a store
+// writes 128 bytes of four rows; 16 bytes of 32 rows took 4000 clocks an item.
 template <int N>
 __device__ __forceinline__ bool store_row(uint32_t ocol, bool there, bool sees, float g,
-                                       __nv_bfloat16* o, uint64_t* o_free)
+                                          __nv_bfloat16* o, long long at, uint64_t* o_free)
 {
+  const uint32_t lane = lane_id();
   bool nan = false;
 #pragma unroll
-  for (int c4 = 0; c4 < N / 32; ++c4) {
-    uint32_t v[32];
-    tmem_ld32(ocol + (uint32_t)(c4 * 32), v);          // whatever it holds, where no key was seen
-    tmem_wait_ld();
-    if (there && c4 + 1 == N / 32) {
+  for (int c8 = 0; c8 < N / 64; ++c8) {
+    uint32_t w[8][4];                                  // eight pieces of 8 columns
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[32];
+      tmem_ld32(ocol + (uint32_t)(c8 * 64 + h * 32), v);   // whatever it holds, where no key was seen
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const float x = sees ? __uint_as_float(v[e]) * g : 0.0f;
+        nan |= x != x;
+        v[e] = __float_as_uint(x);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        w[h * 4 + e / 4][e % 4] = pack_bf16(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+    }
+    if (there && c8 + 1 == N / 64) {
       tc_fence_before();
       __syncwarp();
-      if (lane_id() == 0) mbar_arrive(o_free);
+      if (lane == 0) mbar_arrive(o_free);
     }
+    // piece k of lane i becomes piece i of lane k, in eights
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const float x = sees ? __uint_as_float(v[e]) * g : 0.0f;
-      nan |= x != x;
-      v[e] = __float_as_uint(x);
-    }
-    if (o != nullptr) {
+    for (int s = 4; s > 0; s >>= 1) {
+      const bool up = (lane & (uint32_t)s) != 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint4 q4;
-        q4.x = pack_bf16(__uint_as_float(v[8 * e + 0]), __uint_as_float(v[8 * e + 1]));
-        q4.y = pack_bf16(__uint_as_float(v[8 * e + 2]), __uint_as_float(v[8 * e + 3]));
-        q4.z = pack_bf16(__uint_as_float(v[8 * e + 4]), __uint_as_float(v[8 * e + 5]));
-        q4.w = pack_bf16(__uint_as_float(v[8 * e + 6]), __uint_as_float(v[8 * e + 7]));
-        *reinterpret_cast<uint4*>(o + c4 * 32 + 8 * e) = q4;
+      for (int k = 0; k < 8; ++k) {
+        if ((k & s) != 0) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[k][e] : w[k | s][e], s);
+          if (up) w[k][e] = got;
+          else w[k | s][e] = got;
+        }
       }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const long long to = __shfl_sync(0xffffffffu, at, (int)(lane & 24u) + k);
+      if (to >= 0)
+        *reinterpret_cast<uint4*>(o + to + c8 * 64 + (lane & 7u) * 8) =
+            make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
     }
   }
   return nan;
@@ -708,11 +737,14 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
         tmem_ld32(scol + (uint32_t)(hh * 64 + 32), b);
         tmem_wait_ld();
         if (j0 < all_lo || j0 + kKeys > all_hi) {
+          // bit e of (ma, mb): this row sees score e; one test a score, where two
+          // comparisons took 1500 clocks a tile
           const int from = lo - j0 - hh * 64, to = hi - j0 - hh * 64;
+          const uint32_t ma = bits_from_to(from, to), mb = bits_from_to(from - 32, to - 32);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            if (e < from || e >= to) a[e] = 0xff800000u;             // -inf
-            if (32 + e < from || 32 + e >= to) b[e] = 0xff800000u;
+            a[e] = (ma >> e) & 1u ? a[e] : 0xff800000u;              // -inf
+            b[e] = (mb >> e) & 1u ? b[e] : 0xff800000u;
           }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -796,8 +828,10 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
       const bool valid_row = r < p.tq * p.group && tok < w->nq;
       const int row = w->row0 + tok, head = w->head * p.group + r % p.group;
       const float g = 1.0f / l_row;
-      __nv_bfloat16* orow = p.o + (size_t)row * p.ldo + (size_t)head * D + hh * (D / kSplit);
-      const bool nan = store_row<D / kSplit>(ocol, nt > 0, sees, g, valid_row ? orow : nullptr, &o_free[t]);
+      const long long at = (long long)row * p.ldo + (long long)head * D + hh * (D / kSplit);
+      const bool nan = store_row<D / kSplit>(ocol, nt > 0, sees, g, p.o, valid_row ? at : -1,
+                                             &o_free[t]);
+      __syncwarp();                                    // repair_row follows on these stores
       uint32_t bad = __ballot_sync(0xffffffffu, nan && valid_row);
       while (bad != 0) {
         const int src = __ffs((int)bad) - 1;
