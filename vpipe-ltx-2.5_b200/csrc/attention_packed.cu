@@ -67,12 +67,22 @@ enum : int {
   PERR_ITEM = 0x6A,
 };
 
-template <int D>
+// Width 128 has two forms.  Wide: two query tiles a CTA, so that K and V are read
+// once for 256 rows; a tile's softmax (1980 clocks) and its products (1490) follow
+// each other, 3720 clocks for both tiles' 128 keys.  Narrow: one tile and three
+// score buffers, two groups of softmax warps by turns, 1525 clocks for one tile's
+// 128 keys; half the rows an item.  Under the power cap the wide form runs long
+// prompts faster all the same (528 against 544 us, 8192 tokens, at 1.69 against
+// 1.55 GHz), so the narrow one takes calls whose wide items would not fill the SMs.
+template <int D, bool NARROW>
 struct PkCfg {
-  static constexpr int kTiles = D == 64 ? 4 : D == 128 ? 2 : 1;   // query tiles of a CTA
+  static_assert(D == 128 || !NARROW, "forms");
+  static constexpr int kTiles = D == 64 ? 4 : D == 128 && !NARROW ? 2 : 1;  // query tiles of a CTA
   static constexpr int kKeys = D == 64 ? 64 : 128;     // keys of a tile
-  static constexpr int kSplit = kKeys / 64;            // softmax threads of a row
-  static constexpr int kGroup = 4 * kSplit;            // softmax warps of a query tile
+  static constexpr int kBufs = D == 256 ? 2 : NARROW ? 3 : 1;     // score buffers of a query tile
+  static constexpr int kSplit = kKeys / 64;            // softmax threads of a row, and
+  static constexpr int kAlt = NARROW ? 2 : 1;          // groups that take key tiles in turn
+  static constexpr int kGroup = 4 * kSplit * kAlt;     // softmax warps of a query tile
   static constexpr int kThreads = 128 + 32 * kGroup * kTiles;
   static constexpr int kQAtom = kRows * 128;           // 128 rows x 128 B (64 dims)
   static constexpr int kQTile = (D / 64) * kQAtom;
@@ -81,16 +91,20 @@ struct PkCfg {
   static constexpr int kParts = D == 256 ? 2 : 1;
   static constexpr int kKAtom = kKeys * 128;
   static constexpr int kSlot = (D / 64) * kKAtom / kParts;
-  static constexpr int kSlots = D == 64 ? 16 : (D == 128 ? 4 : 5);
+  static constexpr int kSlots = D == 64 ? 16 : D == 128 && !NARROW ? 4 : 5;
   static constexpr int kVKeys = kKeys / kParts;        // keys of a V slot
-  // row maxima of the two half-row warps: [tile][parity][half][row] f32
-  static constexpr int kMaxBytes = kSplit == 2 ? kTiles * 4 * kRows * 4 : 0;
-  static constexpr int kBars = 2 * kSlots + 4 * (kTiles > 1 ? kTiles : 2) + 8;
+  // row maxima and sums on their way between the threads of a row:
+  // [group][parity][half][row], and the maxima handed from group to group
+  static constexpr int kGroups = kTiles * kAlt;
+  static constexpr int kMaxBytes =
+      kSplit == 1 ? 0 : (kGroups * 4 + (kAlt == 2 ? 4 : 0)) * kRows * 4;
+  static constexpr int kScores = kTiles * kBufs;       // score buffers
+  static constexpr int kBars = 2 * kSlots + 2 * kScores + 4 * kTiles + 8 + (kAlt == 2 ? 16 : 0);
   static constexpr int kBarBytes = (kBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kSmem = kTiles * kQTile + kSlots * kSlot + kMaxBytes + kBarBytes + 256;
   static constexpr uint32_t kOCol = 0;                 // O_t at t * D
-  static constexpr uint32_t kSCol = kTiles * D;        // score buffers: one a tile, two for one
-  static_assert(kSCol + (kTiles > 1 ? kTiles : 2) * kKeys <= 512, "TMEM columns");
+  static constexpr uint32_t kSCol = kTiles * D;        // tile t's buffer i at t * kBufs + i
+  static_assert(kSCol + kScores * kKeys <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -322,38 +336,43 @@ __device__ __forceinline__ int next_index(const void* answer)
   return ok != 0 ? (int)x : -1;
 }
 
-template <int D>
-__global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
+template <int D, bool NARROW>
+__global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     pk_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ PkParams p)
 {
-  using C = PkCfg<D>;
-  constexpr int T = C::kTiles, R = C::kSlots, B = T > 1 ? T : 2, kKeys = C::kKeys;
+  using C = PkCfg<D, NARROW>;
+  constexpr int T = C::kTiles, R = C::kSlots, NB = C::kBufs, kKeys = C::kKeys;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* s_q = smem_raw;                             // tile t at t * kQTile
   uint8_t* s_ring = s_q + T * C::kQTile;
-  float (*s_mx)[2][2][kRows] =                         // [tile][parity][half][row]
+  float (*s_mx)[2][2][kRows] =                         // [group][parity][half][row]
       reinterpret_cast<float (*)[2][2][kRows]>(s_ring + R * C::kSlot);
+  float (*s_m)[2][kRows] =                             // [group][half][row]
+      reinterpret_cast<float (*)[2][kRows]>(s_mx + C::kGroups);
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_ring + R * C::kSlot + C::kMaxBytes);
   uint64_t* q_full = bars;
   uint64_t* q_empty = q_full + 1;
   uint64_t* full = q_empty + 1;
   uint64_t* empty = full + R;
   uint64_t* s_full = empty + R;
-  uint64_t* p_full = s_full + B;
-  uint64_t* o_done = p_full + B;
-  uint64_t* o_free = o_done + B;
-  uint64_t* item_full = o_free + B;
+  uint64_t* p_full = s_full + C::kScores;
+  uint64_t* o_done = p_full + C::kScores;
+  uint64_t* o_free = o_done + 2 * T;                   // o_done: two a tile, by turns
+  uint64_t* o_last = o_free + T;
+  uint64_t* item_full = o_last + T;
   uint64_t* item_empty = item_full + 2;
   uint64_t* asked = item_empty + 2;
   uint64_t* drain = asked + 1;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* m_full = drain + 1;                        // [group][half][lane quarter] (kAlt 2)
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   uint8_t* tail = s_ring + R * C::kSlot + C::kMaxBytes + C::kBarBytes;
   uint8_t* s_answer = tail;                            // 16 bytes
   volatile int* s_fail = reinterpret_cast<volatile int*>(tail + 16);    // one a query tile
+  volatile int* s_swap = s_fail + 2;                   // one a group
   PkItem* s_item = reinterpret_cast<PkItem*>(tail + 32);                // two
   static_assert(32 + 2 * sizeof(PkItem) <= 256, "tail");
 
@@ -372,17 +391,23 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < B; ++i) {
+    for (int i = 0; i < C::kScores; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], C::kGroup);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&o_free[i], C::kGroup);
+      mbar_init(&p_full[i], 4 * C::kSplit);
     }
+    for (int i = 0; i < T; ++i) {
+      mbar_init(&o_done[2 * i], 1);
+      mbar_init(&o_done[2 * i + 1], 1);
+      mbar_init(&o_free[i], 4 * C::kSplit);
+      mbar_init(&o_last[i], 1);
+    }
+    if (C::kAlt == 2)
+      for (int i = 0; i < 16; ++i) mbar_init(&m_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 2 + C::kGroup * T);
-      s_fail[i] = 0;
     }
+    s_fail[0] = s_fail[1] = 0;
     mbar_init(asked, 1);
     mbar_init(drain, 1);
     *s_abort = 0;
@@ -507,11 +532,10 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
             armed_par = (armed_par & ~(1u << st)) | (ph << st);
           }
         };
-        load(false, 0);
+        for (int j = 0; ok && j < min(NB, n); ++j) load(false, j);
         for (int j = 0; ok && j < n; ++j) {
-          if (T == 1 && j + 1 < n) load(false, j + 1);
           load(true, j);
-          if (T > 1 && j + 1 < n) load(false, j + 1);
+          if (j + NB < n) load(false, j + NB);
         }
       }
       // Every load lands before the CTA may exit.
@@ -531,14 +555,18 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, s_abort, p.err, PERR_MMA)) != 0;
     };
-    // a ring of slots: the next one and the parity of its round
-    uint32_t slot = 0, round = 0;
-    auto next_slot = [&]() {
-      if (++slot == (uint32_t)R) {
-        slot = 0;
-        round ^= 1u;
+    // a place in the ring of slots and the parity of its round
+    struct Ring {
+      uint32_t slot, round;
+      __device__ __forceinline__ void next()
+      {
+        if (++slot == (uint32_t)R) {
+          slot = 0;
+          round ^= 1u;
+        }
       }
     };
+    Ring ring = {0, 0};
     const uint64_t q_desc = sdesc_k128_sw128(smem_u32(s_q));
     const uint64_t k_desc = sdesc_k128_sw128(smem_u32(s_ring));
     const uint64_t v_desc = sdesc_mn_sw128(smem_u32(s_ring), C::kVKeys * 128);
@@ -586,94 +614,86 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
       ok = wait(q_full, with_keys & 1u);
       if (!ok) break;
       ++with_keys;
-      if constexpr (T > 1) {
-        ok = wait(&full[slot], round);
-        if (!ok) break;
-        tc_fence_after();
+      // scores of key tile j for every query tile that has it, from the slots at k
+      auto scores = [&](int t, int j, Ring k, bool first) {
+        const uint32_t buf = (uint32_t)(t * NB) + ((step[t] + (uint32_t)j) % (uint32_t)NB);
+#pragma unroll
+        for (int part = 0; part < C::kParts; ++part) {
+          if (ok && first) ok = wait(&full[k.slot], k.round);
+          if (!ok) return;
+          tc_fence_after();
+          issue_s(t, buf, k.slot, part);
+          if (T == 1) umma_commit_by(lead, &empty[k.slot]);
+          k.next();
+        }
+        umma_commit_by(lead, &s_full[buf]);
+      };
+      auto release = [&](Ring k) {                     // with one query tile each use does it
+        if (T > 1) umma_commit_by(lead, &empty[k.slot]);
+      };
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        if (!ok || j >= n) continue;
+        bool first = true;
 #pragma unroll
         for (int t = 0; t < T; ++t)
-          if (tiles[t] > 0) {
-            issue_s(t, (uint32_t)t, slot, 0);
-            umma_commit_by(lead, &s_full[t]);
+          if (ok && j < tiles[t]) {
+            scores(t, j, ring, first);
+            first = false;
           }
-        umma_commit_by(lead, &empty[slot]);
-        if (n == 1) umma_commit_by(lead, q_empty);
-        next_slot();
-        for (int j = 0; ok && j < n; ++j) {
-          const uint32_t av = slot, av_round = round;  // V_j, then K_{j+1}
-          next_slot();
-          const uint32_t ak = slot, ak_round = round;
-          const bool more = j + 1 < n;
-          bool have_v = false, have_k = false;
+        if (!ok) continue;
+        release(ring);
 #pragma unroll
-          for (int t = 0; t < T; ++t) {
-            if (!ok || j >= tiles[t]) continue;
-            // P V, then the tile's next S (in order: the S MMA overwrites the
-            // buffer only after this P V has read P from it); an item's first P V
-            // overwrites O, which the softmax must have read
-            ok = wait(&p_full[t], step[t] & 1u);
-            ++step[t];
-            if (ok && j == 0) ok = wait(&o_free[t], (opened[t]++ & 1u) ^ 1u);
-            if (ok && !have_v) ok = wait(&full[av], av_round);
-            have_v = true;
-            if (!ok) continue;
-            tc_fence_after();
-            issue_pv(t, (uint32_t)t, av, 0, j == 0);
-            umma_commit_by(lead, &o_done[t]);
-            if (j + 1 < tiles[t]) {
-              if (!have_k) ok = wait(&full[ak], ak_round);
-              have_k = true;
-              if (!ok) continue;
-              tc_fence_after();
-              issue_s(t, (uint32_t)t, ak, 0);
-              umma_commit_by(lead, &s_full[t]);
-            }
-          }
-          if (!ok) break;
-          umma_commit_by(lead, &empty[av]);
-          if (more) {
-            umma_commit_by(lead, &empty[ak]);
-            next_slot();
-          }
-          if (j + 2 == n) umma_commit_by(lead, q_empty);
-        }
-      } else {
-        // S_0, then S_{j+1} and P_j V_j by turns
-        const uint32_t base = step[0];
-        for (int j = -1; ok && j < n; ++j) {
-          if (j + 1 < n) {
-            const uint32_t b = (base + (uint32_t)(j + 1)) & 1u;
+        for (int part = 0; part < C::kParts; ++part) ring.next();
+        if (j + 1 == n) umma_commit_by(lead, q_empty);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const Ring v = ring;                           // V_j, then K_{j + NB}
 #pragma unroll
-            for (int part = 0; part < C::kParts; ++part) {
-              if (ok) ok = wait(&full[slot], round);
-              if (!ok) continue;
-              tc_fence_after();
-              issue_s(0, b, slot, part);
-              umma_commit_by(lead, &empty[slot]);
-              next_slot();
-            }
-            if (!ok) break;
-            umma_commit_by(lead, &s_full[b]);
-            if (j + 2 == n) umma_commit_by(lead, q_empty);
-          }
-          if (j < 0) continue;
-          const uint32_t at = base + (uint32_t)j;
-          ok = wait(&p_full[at & 1u], (at >> 1) & 1u);
-          if (ok && j == 0) ok = wait(&o_free[0], (opened[0]++ & 1u) ^ 1u);
+        for (int part = 0; part < C::kParts; ++part) ring.next();
+        const Ring k = ring;
+        const bool more = j + NB < n;
+        bool have_v = false, have_k = false;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          if (!ok || j >= tiles[t]) continue;
+          // P V, then the scores that take its buffer (in order: they overwrite it
+          // only after this P V has read P from it); an item's first P V overwrites
+          // O, which the softmax must have read
+          const uint32_t at = step[t] + (uint32_t)j;
+          const uint32_t buf = (uint32_t)(t * NB) + at % (uint32_t)NB;
+          ok = wait(&p_full[buf], (at / (uint32_t)NB) & 1u);
+          if (ok && j == 0) ok = wait(&o_free[t], (opened[t]++ & 1u) ^ 1u);
+          Ring vv = v;
 #pragma unroll
           for (int part = 0; part < C::kParts; ++part) {
-            if (ok) ok = wait(&full[slot], round);
+            if (ok && !have_v) ok = wait(&full[vv.slot], vv.round);
             if (!ok) continue;
             tc_fence_after();
-            issue_pv(0, at & 1u, slot, part, j == 0);
-            umma_commit_by(lead, &empty[slot]);
-            next_slot();
+            issue_pv(t, buf, vv.slot, part, j == 0);
+            if (T == 1) umma_commit_by(lead, &empty[vv.slot]);
+            vv.next();
           }
-          if (!ok) break;
-          umma_commit_by(lead, &o_done[0]);
+          have_v = true;
+          if (!ok) continue;
+          umma_commit_by(lead, &o_done[2 * t + (int)(at & 1u)]);
+          if (j + 1 == tiles[t]) umma_commit_by(lead, &o_last[t]);
+          if (j + NB < tiles[t]) {
+            scores(t, j + NB, k, !have_k);
+            have_k = true;
+          }
         }
-        step[0] = base + (uint32_t)n;
+        if (!ok) break;
+        release(v);
+        if (more) {
+          release(k);
+#pragma unroll
+          for (int part = 0; part < C::kParts; ++part) ring.next();
+        }
+        if (j + NB + 1 == n) umma_commit_by(lead, q_empty);
       }
+#pragma unroll
+      for (int t = 0; t < T; ++t) step[t] += (uint32_t)tiles[t];
     }
     umma_commit_by(lead, drain);
     volatile int no_abort = 0;
@@ -681,16 +701,22 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
     __syncwarp();
   } else if (warp >= 4) {
     // ---------------------------------------------------------- softmax
-    // Four warps a tile with a row a thread, or eight: the first four take score
-    // columns [0, 64), the next four [64, 128) of the same rows.
-    constexpr int kSplit = C::kSplit;
+    // Four warps a tile with a row a thread; or eight with two threads a row (hh:
+    // score columns [0, 64) and [64, 128) of a key tile), or two such groups that
+    // take the key tiles in turn (`alt`), so that one's exponentials run under the
+    // other's maxima, stores and waits.
+    constexpr int kSplit = C::kSplit, kAlt = C::kAlt;
     const int t = (warp - 4) / C::kGroup;
     const int hh = ((warp - 4) >> 2) & (kSplit - 1);
-    const int r = (warp & 3) * 32 + (int)lane;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ocol = tmem + lane_base + C::kOCol + (uint32_t)(t * D + hh * (D / kSplit));
+    const int alt = (warp - 4) / (4 * kSplit) & (kAlt - 1);
+    const int gx = t * kAlt + alt;                     // this group, of kGroups
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + (int)lane;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t orow = tmem + lane_base + C::kOCol + (uint32_t)(t * D);
     const float c = p.c;
-    uint32_t step = 0, swap = 0;                       // score tiles, exchanges so far
+    // score tiles of this query tile so far, and exchanges (kSplit 2)
+    uint32_t step = 0, swap = 0, closed = 0;           // closed: items with keys
     bool ok = true;
 #pragma unroll 1
     for (int it = 0;; ++it) {
@@ -699,18 +725,18 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
       // same for all.
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u,
                                                    s_abort, p.err, PERR_SOFTMAX));
-      if (kSplit == 1) {
+      if (kSplit * kAlt == 1) {
         if (!ok) break;
       } else {
         if (!ok && lane == 0) s_fail[t] = 1;
-        named_bar_sync(1 + t, 256);
+        named_bar_sync(1 + t, 32 * C::kGroup);
         if (s_fail[t] != 0) break;
       }
       // the item stays in its place until this role is through with it
       const PkItem* w = &s_item[it & 1];
       if (w->head < 0) break;
       const int nt = w->tiles[t];
-      int j0 = w->first;
+      const int first = w->first;
       // the keys this thread's row sees, and those that all valid rows of the
       // query tile see
       int lo, hi, all_lo, all_hi;
@@ -723,19 +749,22 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
         all_lo = key_low(shift + b_tok, p.window);
         all_hi = key_high(shift + a_tok, w->nk, p.causal);
       }
+      // m_run: what this thread's sum refers to.  kAlt 2: the row's maximum goes
+      // from group to group with the key tiles (s_mx[t][1][group]).
       float m_run = -INFINITY, l_run = 0.0f;
 #pragma unroll 1
-      for (int i = 0; i < nt; ++i, ++step, ++swap, j0 += kKeys) {
-        const int sb = T > 1 ? t : (int)(step & 1u);
-        const uint32_t ph = T > 1 ? step & 1u : (step >> 1) & 1u;
+      for (int i = kAlt == 2 ? (int)((step ^ (uint32_t)alt) & 1u) : 0; i < nt; i += kAlt) {
+        const uint32_t at = step + (uint32_t)i;        // this score tile
+        const int sb = t * NB + (int)(at % (uint32_t)NB);
         const uint32_t scol = tmem + lane_base + C::kSCol + (uint32_t)(sb * kKeys);
-        ok = __all_sync(0xffffffffu,
-                        ok && mbar_wait(&s_full[sb], ph, s_abort, p.err, PERR_SOFTMAX));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&s_full[sb], (at / (uint32_t)NB) & 1u, s_abort,
+                                                     p.err, PERR_SOFTMAX));
         uint32_t a[32], b[32];
         tc_fence_after();
         tmem_ld32(scol + (uint32_t)(hh * 64), a);
         tmem_ld32(scol + (uint32_t)(hh * 64 + 32), b);
         tmem_wait_ld();
+        const int j0 = first + i * kKeys;
         if (j0 < all_lo || j0 + kKeys > all_hi) {
           // bit e of (ma, mb): this row sees score e; one test a score, where two
           // comparisons took 1500 clocks a tile
@@ -755,27 +784,49 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
           m4[2] = max3f(m4[2], __uint_as_float(b[e]), __uint_as_float(b[e + 1]));
           m4[3] = max3f(m4[3], __uint_as_float(b[e + 2]), __uint_as_float(b[e + 3]));
         }
-        // the row's max over both halves: exchange through shared memory (both
-        // halves have their scores in registers after this barrier, so either
-        // may then overwrite the TMEM columns with P)
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        float m_old = m_run;                           // what O refers to
         if (kSplit == 2) {
-          s_mx[t][swap & 1u][hh][r] = mx;
-          named_bar_sync(1 + t, 256);
-          mx = fmaxf(s_mx[t][swap & 1u][0][r], s_mx[t][swap & 1u][1][r]);
+          // the row's max over both halves: exchange through shared memory (both
+          // halves have their scores in registers after this barrier, so either
+          // may then overwrite the TMEM columns with P)
+          s_mx[gx][swap & 1u][hh][r] = mx;
+          named_bar_sync(3 + gx, 256);
+          mx = fmaxf(s_mx[gx][swap & 1u][0][r], s_mx[gx][swap & 1u][1][r]);
+          ++swap;
+        }
+        if (kAlt == 2) {
+          // the maximum that the other group's key tile left
+          if (i == 0) {
+            m_old = -INFINITY;
+          } else {
+            ok = __all_sync(0xffffffffu,
+                            ok && mbar_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
+                                            ((at - 1u) >> 1) & 1u, s_abort, p.err, PERR_SOFTMAX));
+            m_old = s_m[alt ^ 1][hh][r];
+          }
         }
         if (!ok) continue;
         const float m_tile = mx * c;
         // a row's first visible tile sets its maximum; later it moves only when
         // it grows by more than 2^kGrow (until then P stays below 2^kGrow)
-        const bool need = m_tile > m_run + kGrow;
+        const bool need = m_tile > m_old + kGrow;
         const bool rescale = i > 0 && __any_sync(0xffffffffu, need);
-        float f = 1.0f;
-        if (need) {
-          f = fast_exp2(m_run - m_tile);
-          l_run *= f;
-          m_run = m_tile;
+        const float m_new = need ? m_tile : m_old;
+        if (kAlt == 2) {
+          s_m[alt][hh][r] = m_new;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_full[(alt * 2 + hh) * 4 + quarter]);
         }
+        float f = 1.0f;
+        if (need) f = fast_exp2(m_old - m_new);
+        if (kAlt == 2) {
+          // this group's sum may refer to an older maximum than O
+          if (m_run != m_new) l_run *= fast_exp2(m_run - m_new);
+        } else {
+          l_run *= f;
+        }
+        m_run = m_new;
         const float nm = m_run == -INFINITY ? 0.0f : -m_run;
         const unsigned long long c2 = pair2(__float_as_uint(c), __float_as_uint(c));
         const unsigned long long nm2 = pair2(__float_as_uint(nm), __float_as_uint(nm));
@@ -785,19 +836,25 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
         tmem_st32(scol + (uint32_t)(hh * 32), pk);
         const unsigned long long st2 = fadd2(sa, sb2);
         l_run += __uint_as_float((uint32_t)st2) + __uint_as_float((uint32_t)(st2 >> 32));
-        if (rescale)
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&o_done[t], (step - 1u) & 1u, s_abort, p.err, PERR_SOFTMAX));
-        if (rescale && ok) {
-          tc_fence_after();
+        if (rescale) {
+          // All of O but this key tile's part.  Of the barrier's two rounds back the
+          // P V at - 3 is done (these scores came after it), so the parity is plain;
+          // with one barrier P V at - 2, under way or done, would leave it open.
+          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * t + (int)((at - 1u) & 1u)],
+                                                 ((at - 1u) >> 1) & 1u, s_abort, p.err,
+                                                 PERR_SOFTMAX));
+          if (ok) {
+            tc_fence_after();
 #pragma unroll
-          for (int c4 = 0; c4 < D / kSplit / 32; ++c4) {
-            uint32_t v[32];
-            tmem_ld32(ocol + (uint32_t)(c4 * 32), v);
-            tmem_wait_ld();
+            for (int c4 = 0; c4 < D / kSplit / 32; ++c4) {
+              uint32_t v[32];
+              const uint32_t oc = orow + (uint32_t)(hh * (D / kSplit) + c4 * 32);
+              tmem_ld32(oc, v);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-            tmem_st32(ocol + (uint32_t)(c4 * 32), v);
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              tmem_st32(oc, v);
+            }
           }
         }
         tmem_wait_st();
@@ -805,40 +862,65 @@ __global__ void __launch_bounds__(PkCfg<D>::kThreads, 1)
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(&p_full[sb]);
       }
-      // the row's sum over both halves
+      // the row's sum over its threads, under the last maximum
       float l_row = l_run;
-      if (kSplit == 2) {
-        s_mx[t][swap & 1u][hh][r] = l_run;
-        named_bar_sync(1 + t, 256);
-        l_row = s_mx[t][swap & 1u][0][r] + s_mx[t][swap & 1u][1][r];
+      if (kAlt == 2 && nt > 0) {
+        const uint32_t end = step + (uint32_t)nt - 1u;
+        float m_end = m_run;
+        if ((int)(end & 1u) != alt) {
+          ok = __all_sync(0xffffffffu,
+                          ok && mbar_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
+                                          (end >> 1) & 1u, s_abort, p.err, PERR_SOFTMAX));
+          m_end = s_m[alt ^ 1][hh][r];
+        }
+        if (m_run != m_end) l_row *= fast_exp2(m_run - m_end);
+      }
+      if (kSplit * kAlt > 1) {
+        // (the last exchange's reads of this place were before the barrier at the
+        // start of this item or an exchange in it)
+        s_mx[gx][swap & 1u][hh][r] = l_row;
+        if (kAlt == 2) s_swap[alt] = (int)(swap & 1u);
+        named_bar_sync(1 + t, 32 * C::kGroup);
+        l_row = s_mx[gx][swap & 1u][0][r] + s_mx[gx][swap & 1u][1][r];
+        if (kAlt == 2) {
+          const int at = s_swap[alt ^ 1];
+          l_row += s_mx[alt ^ 1][at][0][r] + s_mx[alt ^ 1][at][1][r];
+        }
         ++swap;
       }
-      // A wait on a parity must not be two phases ahead.  With several tiles the last
-      // scores followed the last P V but one; with one tile they ran before it.
-      if (T == 1 && ok && nt > 1)
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(&o_done[t], (step - 2u) & 1u, s_abort, p.err, PERR_SOFTMAX));
-      if (ok && nt > 0)
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(&o_done[t], (step - 1u) & 1u, s_abort, p.err, PERR_SOFTMAX));
+      step += (uint32_t)nt;
+      // The rows go out; of two groups the one without the last key tile does it.
+      // (All of O is waited for by a barrier of its own: by o_done the P V before the
+      // last may be under way still, or both be done, and a parity tells neither.)
+      const bool stores = kAlt == 1 || (nt > 0 ? (int)((step - 1u) & 1u) != alt : alt == 0);
+      if (nt > 0) {
+        if (stores)
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_last[t], closed & 1u, s_abort, p.err,
+                                                       PERR_SOFTMAX));
+        ++closed;
+      }
       if (!ok) continue;
-      tc_fence_after();
-      const bool sees = nt > 0 && hi > lo;
-      const int tok = w->tok0 + t * p.tq + r / p.group;
-      const bool valid_row = r < p.tq * p.group && tok < w->nq;
-      const int row = w->row0 + tok, head = w->head * p.group + r % p.group;
-      const float g = 1.0f / l_row;
-      const long long at = (long long)row * p.ldo + (long long)head * D + hh * (D / kSplit);
-      const bool nan = store_row<D / kSplit>(ocol, nt > 0, sees, g, p.o, valid_row ? at : -1,
-                                             &o_free[t]);
-      __syncwarp();                                    // repair_row follows on these stores
-      uint32_t bad = __ballot_sync(0xffffffffu, nan && valid_row);
-      while (bad != 0) {
-        const int src = __ffs((int)bad) - 1;
-        bad &= bad - 1;
-        repair_row<D, D / kSplit>(p, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src),
-                      w->head, w->key0, __shfl_sync(0xffffffffu, lo, src),
-                      __shfl_sync(0xffffffffu, hi, src), hh * (D / kSplit));
+      if (stores) {
+        tc_fence_after();
+        constexpr int kCols = D / kSplit;
+        const bool sees = nt > 0 && hi > lo;
+        const int tok = w->tok0 + t * p.tq + r / p.group;
+        const bool valid_row = r < p.tq * p.group && tok < w->nq;
+        const int row = w->row0 + tok, head = w->head * p.group + r % p.group;
+        const float g = 1.0f / l_row;
+        const long long to = (long long)row * p.ldo + (long long)head * D + hh * kCols;
+        const bool nan = store_row<kCols>(orow + (uint32_t)(hh * kCols), nt > 0, sees, g, p.o,
+                                          valid_row ? to : -1, &o_free[t]);
+        __syncwarp();                                  // repair_row follows on these stores
+        uint32_t bad = __ballot_sync(0xffffffffu, nan && valid_row);
+        while (bad != 0) {
+          const int src = __ffs((int)bad) - 1;
+          bad &= bad - 1;
+          repair_row<D, kCols>(p, __shfl_sync(0xffffffffu, row, src),
+                               __shfl_sync(0xffffffffu, head, src), w->head, w->key0,
+                               __shfl_sync(0xffffffffu, lo, src),
+                               __shfl_sync(0xffffffffu, hi, src), hh * kCols);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[it & 1]);
@@ -876,10 +958,10 @@ bool pk_encode(CUtensorMap* map, const __nv_bfloat16* x, int D, int heads, int r
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, bool NARROW>
 int pk_launch(const PackedAttention& a, int* err, cudaStream_t s)
 {
-  using C = PkCfg<D>;
+  using C = PkCfg<D, NARROW>;
   PkParams p;
   memset(&p, 0, sizeof(p));
   p.q = a.q;
@@ -913,20 +995,24 @@ int pk_launch(const PackedAttention& a, int* err, cudaStream_t s)
       (long long)slot_count(a.rows, a.seqs, C::kTiles * p.tq, 1) * a.kv_heads;
   if (grid > INT_MAX) return -2;
   static std::atomic<unsigned long long> attr{0};
-  if (!smem_limit_once(pk_attention_kernel<D>, C::kSmem, attr)) return -1;
-  launch_k(pk_attention_kernel<D>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1, mq, mk,
+  if (!smem_limit_once(pk_attention_kernel<D, NARROW>, C::kSmem, attr)) return -1;
+  launch_k(pk_attention_kernel<D, NARROW>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1, mq, mk,
            mv, p);
   return launched();
 }
 
 }  // namespace
 
-int launch_attention_packed(const PackedAttention& a, int* err, cudaStream_t s)
+int launch_attention_packed(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
 {
   switch (a.head_dim) {
-    case 64: return pk_launch<64>(a, err, s);
-    case 128: return pk_launch<128>(a, err, s);
-    case 256: return pk_launch<256>(a, err, s);
+    case 64: return pk_launch<64, false>(a, err, s);
+    case 128: {
+      const int tq = kRows / (a.heads / a.kv_heads);
+      const long long wide = (long long)slot_count(a.rows, a.seqs, 2 * tq, 1) * a.kv_heads;
+      return wide <= num_sms ? pk_launch<128, true>(a, err, s) : pk_launch<128, false>(a, err, s);
+    }
+    case 256: return pk_launch<256, false>(a, err, s);
     default: return -2;
   }
 }

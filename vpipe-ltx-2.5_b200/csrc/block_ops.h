@@ -141,7 +141,7 @@ struct PackedAttention {
   int causal = 1, window = 0;
   float scale = 0.0f;
 };
-int launch_attention_packed(const PackedAttention& a, int* err, cudaStream_t s);
+int launch_attention_packed(const PackedAttention& a, int num_sms, int* err, cudaStream_t s);
 
 // The 8-bit key/value cache (kv8.cu).  Codes int8 [pages][kv_heads][64][D],
 // bf16 scales [pages][kv_heads]; head_dim 64, 128 or 256.

@@ -724,7 +724,7 @@ int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const void* k, in
     const int rc = ltx25::check_attention_packed(a, &e);
     if (rc != LTX_OK) return fail(ctx, rc, e);
     if (seqs == 0 || rows == 0) return LTX_OK;
-    if (ltx::launch_attention_packed(a, ctx->ops.err_word(), S(stream)) != 0)
+    if (ltx::launch_attention_packed(a, ctx->ops.num_sms(), ctx->ops.err_word(), S(stream)) != 0)
       return fail(ctx, LTX_E_CUDA, "attention_packed launch failed");
     return LTX_OK;
   });
