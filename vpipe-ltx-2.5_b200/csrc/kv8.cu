@@ -54,50 +54,136 @@ struct KvPages {
   int* err;
 };
 
+// A run of new tokens on one page.
 struct KvSpan {
-  int row, from, count;           // packed row of the first token, its slot, tokens
-  size_t page;                    // page * kv_heads + head
+  int seq, row, block;            // sequence, packed row of the first token, its page's place
+  int from, count;                // slot of the first token, tokens
 };
 
-// The tokens of one page that work slot `slot` covers, false where it has none.
-// Every thread of the block calls it.
-__device__ __forceinline__ bool kv_span(const KvPages& p, int slot, int head, KvSpan* out)
+// The tokens of the page that work slot `slot` covers; count 0 where it has none.
+// Whole warps call it.  Up to 32 sequences each lane looks at one, so that one
+// round of loads answers.
+__device__ __forceinline__ KvSpan kv_span(const KvPages& p, int slot)
 {
-  const int s = find_seq(p.cu, p.seqs, p.rows, kPage, 2, slot);
-  const int row0 = clamp_int(p.cu[s], 0, p.rows);
-  const int n = clamp_int(p.cu[s + 1], row0, p.rows) - row0;
+  KvSpan w;
+  int s, row0, end, start;
+  if (p.seqs <= 32) {
+    const int lane = (int)lane_id();
+    int a = 0, b = 0, c = 0;
+    if (lane < p.seqs) {
+      a = p.cu[lane];
+      b = p.cu[lane + 1];
+      c = p.starts[lane];
+    }
+    a = clamp_int(a, 0, p.rows);
+    const bool below = lane == 0 || (lane < p.seqs && slot_base(a, lane, kPage, 2) <= slot);
+    s = 31 - __clz((int)__ballot_sync(0xffffffffu, below));
+    row0 = __shfl_sync(0xffffffffu, a, s);
+    end = __shfl_sync(0xffffffffu, b, s);
+    start = __shfl_sync(0xffffffffu, c, s);
+  } else {
+    s = find_seq(p.cu, p.seqs, p.rows, kPage, 2, slot);
+    row0 = clamp_int(p.cu[s], 0, p.rows);
+    end = p.cu[s + 1];
+    start = p.starts[s];
+  }
+  const int n = clamp_int(end, row0, p.rows) - row0;
   const int i = slot - slot_base(row0, s, kPage, 2);
-  const int start = p.starts[s];
-  if (n == 0 || i < 0) return false;
-  const int cap = p.table_ld * kPage;
-  if (!span_ok(start, n, cap)) {
+  w.seq = s;
+  w.count = 0;
+  if (n == 0 || i < 0) return w;
+  if (!span_ok(start, n, p.table_ld * kPage)) {
     if (threadIdx.x == 0) atomicCAS(p.err, 0, KERR_PLACE);
-    return false;
+    return w;
   }
   const PageSpan span = page_span(start, n, i);
-  if (span.b <= span.a) return false;
-  const int page = p.table[(size_t)s * p.table_ld + span.block];
-  if (!page_ok(page, p.pages)) {
-    if (threadIdx.x == 0) atomicCAS(p.err, 0, KERR_PLACE);
-    return false;
-  }
-  out->row = row0 + (span.a - start);
-  out->from = span.a - span.block * kPage;
-  out->count = span.b - span.a;
-  out->page = (size_t)page * p.kv_heads + head;
-  return true;
+  w.block = span.block;
+  w.row = row0 + (span.a - start);
+  w.from = span.a - span.block * kPage;
+  w.count = max(0, span.b - span.a);
+  return w;
 }
 
-constexpr int kAppendThreads = 256;
+// The span's page, or -1 where the table names none.
+__device__ __forceinline__ int kv_page(const KvPages& p, const KvSpan& w)
+{
+  const int page = p.table[(size_t)w.seq * p.table_ld + w.block];
+  if (page_ok(page, p.pages)) return page;
+  if ((threadIdx.x & 31) == 0) atomicCAS(p.err, 0, KERR_PLACE);
+  return -1;
+}
 
-// One page, one head, keys (blockIdx.z 0) or values (1) a block: the new rows
-// stay in registers between the search for their maximum and their rounding,
-// so they are read once.
+__device__ __forceinline__ uint32_t max_bits(uint4 v)
+{
+  const uint32_t a = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+  const uint32_t b = __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu);
+  return __vmaxu2(a, b);
+}
+
+// The scale of a page and head once values of magnitude `most` join it.  bf16
+// magnitudes order like their bits; a NaN or infinity is above 0x7f7f and makes the
+// scale NaN.
+__device__ __forceinline__ uint32_t joined_scale(uint32_t most, uint32_t was, bool held)
+{
+  const uint32_t now = most > 0x7f7fu ? 0x7fc0u : page_scale(most);
+  return held ? max(now, was) : now;
+}
+
+// The page's own codes, brought to a grown scale: c * was / now, a quotient of 15
+// by 8 bits, decided by the correctly rounded f32 division.
+__device__ __forceinline__ void rescale_codes(int8_t* codes, int count4, uint32_t was, uint32_t now,
+                                              int at, int step)
+{
+  const float s0 = bf16_bits(was), s1 = bf16_bits(now);
+  for (int i = at; i < count4; i += step) {
+    char4 c = reinterpret_cast<char4*>(codes)[i];
+    c.x = (signed char)__float2int_rn(__fdiv_rn((float)c.x * s0, s1));
+    c.y = (signed char)__float2int_rn(__fdiv_rn((float)c.y * s0, s1));
+    c.z = (signed char)__float2int_rn(__fdiv_rn((float)c.z * s0, s1));
+    c.w = (signed char)__float2int_rn(__fdiv_rn((float)c.w * s0, s1));
+    reinterpret_cast<char4*>(codes)[i] = c;
+  }
+}
+
+// x / s to the nearest integer, ties to even, for the bf16 values x and scale s:
 //   t = x / s by one product with 1 / s, within 2^-15 of the quotient;
 //   adding and taking away 1.5 * 2^12 rounds it to a multiple of 2^-11, which
 //   puts a tie back on the tie and leaves all others on their side (2^-9);
 //   adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves
 //   the code in the sum's low byte.
+// 1 / s may not be finite for a tiny s: both are scaled by 2^64 there.
+struct KvCoder {
+  float mul, inv;
+  __device__ __forceinline__ explicit KvCoder(uint32_t scale)
+  {
+    const float s = bf16_bits(scale);
+    const bool none = scale > 0x7f7fu || s == 0.0f;
+    mul = none ? 0.0f : s < 0x1p-64f ? 0x1p64f : 1.0f;
+    inv = none ? 0.0f : __frcp_rn(s * mul);
+  }
+  __device__ __forceinline__ uint32_t one(float x) const
+  {
+    const float t = (x * mul) * inv;
+    const float snapped = __fadd_rn(__fadd_rn(t, 6144.0f), -6144.0f);
+    return __float_as_uint(__fadd_rn(snapped, 12582912.0f));
+  }
+  __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b) const
+  {
+    const uint32_t c0 = one(__uint_as_float(a << 16)), c1 = one(__uint_as_float(a & 0xffff0000u));
+    const uint32_t c2 = one(__uint_as_float(b << 16)), c3 = one(__uint_as_float(b & 0xffff0000u));
+    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
+  }
+  __device__ __forceinline__ uint2 eight(uint4 v) const
+  {
+    return make_uint2(four(v.x, v.y), four(v.z, v.w));
+  }
+};
+
+constexpr int kAppendThreads = 256;
+
+// Many rows: one page, one head, keys (blockIdx.z 0) or values (1) a block.  The new
+// rows stay in registers between the search for their maximum and their rounding,
+// so they are read once; they are on their way before the page is known.
 template <int D>
 __global__ void __launch_bounds__(kAppendThreads)
     kv8_append_kernel(KvPages p, const __nv_bfloat16* k, int ldk, const __nv_bfloat16* v, int ldv)
@@ -108,78 +194,97 @@ __global__ void __launch_bounds__(kAppendThreads)
   __shared__ uint32_t s_most[kAppendThreads / 32];
   pdl_wait();
   pdl_trigger();
-  KvSpan w;
-  if (!kv_span(p, (int)blockIdx.x, (int)blockIdx.y, &w)) return;
+  // heads of a page are neighbours in the grid, as their columns are in a row
+  const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+  const KvSpan w = kv_span(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
+  if (w.count == 0) return;
   const bool val = blockIdx.z != 0;
   const __nv_bfloat16* x = val ? v : k;
   const int ld = val ? ldv : ldk;
-  int8_t* codes = (val ? p.v : p.k) + w.page * (size_t)(kPage * D);
-  uint16_t* scale = (val ? p.vs : p.ks) + w.page;
   const int chunk = (int)threadIdx.x % kChunks, r0 = (int)threadIdx.x / kChunks;
-
   uint4 in[kPasses];
-  uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = r0 + i * kRowsAt;
     in[i] = make_uint4(0, 0, 0, 0);
     if (r < w.count)
       in[i] = *reinterpret_cast<const uint4*>(x + (size_t)(w.row + r) * ld +
-                                              (size_t)blockIdx.y * D + chunk * 8);
-    const uint32_t a = __vmaxu2(in[i].x & 0x7fff7fffu, in[i].y & 0x7fff7fffu);
-    const uint32_t b = __vmaxu2(in[i].z & 0x7fff7fffu, in[i].w & 0x7fff7fffu);
-    most = __vmaxu2(most, __vmaxu2(a, b));
+                                              (size_t)head * D + chunk * 8);
   }
+  const int page = kv_page(p, w);
+  if (page < 0) return;
+  const size_t line = (size_t)page * p.kv_heads + head;
+  int8_t* codes = (val ? p.v : p.k) + line * (size_t)(kPage * D);
+  uint16_t* scale = (val ? p.vs : p.ks) + line;
+  const uint32_t was = *scale;
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) most = __vmaxu2(most, max_bits(in[i]));
   most = max(most & 0xffffu, most >> 16);
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
-  const uint32_t was = *scale;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kAppendThreads / 32; ++i) most = max(most, s_most[i]);
-
-  // bf16 magnitudes order like their bits; a NaN or infinity is above 0x7f7f
-  // and makes the page's scale NaN
-  uint32_t now = most > 0x7f7fu ? 0x7fc0u : page_scale(most);
-  if (w.from > 0) now = max(now, was);
-  const bool bad = now > 0x7f7fu;
-  if (w.from > 0 && now != was && !bad) {
-    // the page's own codes, brought to the grown scale: c * was / now, a
-    // quotient of 15 by 8 bits, decided by the correctly rounded f32 division
-    const float s0 = bf16_bits(was), s1 = bf16_bits(now);
-    for (int i = (int)threadIdx.x; i < w.from * (D / 4); i += kAppendThreads) {
-      char4 c = reinterpret_cast<char4*>(codes)[i];
-      c.x = (signed char)__float2int_rn(__fdiv_rn((float)c.x * s0, s1));
-      c.y = (signed char)__float2int_rn(__fdiv_rn((float)c.y * s0, s1));
-      c.z = (signed char)__float2int_rn(__fdiv_rn((float)c.z * s0, s1));
-      c.w = (signed char)__float2int_rn(__fdiv_rn((float)c.w * s0, s1));
-      reinterpret_cast<char4*>(codes)[i] = c;
-    }
-  }
+  const uint32_t now = joined_scale(most, was, w.from > 0);
+  if (w.from > 0 && now != was && now <= 0x7f7fu)
+    rescale_codes(codes, w.from * (D / 4), was, now, (int)threadIdx.x, kAppendThreads);
   if (threadIdx.x == 0 && (w.from == 0 || now != was)) *scale = (uint16_t)now;
-
-  // 1 / s may not be finite for a tiny s: both are scaled by 2^64 there
-  const float s = bf16_bits(now);
-  const float pre = s < 0x1p-64f ? 0x1p64f : 1.0f;
-  const float inv = bad || s == 0.0f ? 0.0f : __frcp_rn(s * pre);
-  const float mul = bad ? 0.0f : pre;
-  auto code = [&](float f) {
-    const float t = (f * mul) * inv;
-    const float snapped = __fadd_rn(__fadd_rn(t, 6144.0f), -6144.0f);
-    return __float_as_uint(__fadd_rn(snapped, 12582912.0f));
-  };
-  auto four = [&](uint32_t a, uint32_t b) {
-    const uint32_t c0 = code(__uint_as_float(a << 16)), c1 = code(__uint_as_float(a & 0xffff0000u));
-    const uint32_t c2 = code(__uint_as_float(b << 16)), c3 = code(__uint_as_float(b & 0xffff0000u));
-    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
-  };
+  const KvCoder coder(now);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = r0 + i * kRowsAt;
     if (r >= w.count) break;
-    uint2 c = make_uint2(0, 0);
-    if (!bad) c = make_uint2(four(in[i].x, in[i].y), four(in[i].z, in[i].w));
-    *reinterpret_cast<uint2*>(codes + (size_t)(w.from + r) * D + chunk * 8) = c;
+    *reinterpret_cast<uint2*>(codes + (size_t)(w.from + r) * D + chunk * 8) =
+        now > 0x7f7fu ? make_uint2(0, 0) : coder.eight(in[i]);
+  }
+}
+
+// Few rows (a token for each sequence): a block a page, a warp for each head's keys
+// or values by turns.
+template <int D>
+__global__ void __launch_bounds__(kAppendThreads)
+    kv8_append_few_kernel(KvPages p, const __nv_bfloat16* k, int ldk, const __nv_bfloat16* v,
+                          int ldv)
+{
+  constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;
+  pdl_wait();
+  pdl_trigger();
+  const KvSpan w = kv_span(p, (int)blockIdx.x);
+  if (w.count == 0) return;
+  const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+  const int chunk = lane % kChunks, r0 = lane / kChunks;
+  int page = -2;
+  for (int i = warp; i < 2 * p.kv_heads; i += kAppendThreads / 32) {
+    const bool val = i >= p.kv_heads;
+    const int head = val ? i - p.kv_heads : i;
+    const __nv_bfloat16* x = (val ? v : k) + (size_t)w.row * (val ? ldv : ldk) + (size_t)head * D +
+                             chunk * 8;
+    const int ld = val ? ldv : ldk;
+    uint4 first = make_uint4(0, 0, 0, 0);
+    if (r0 < w.count) first = *reinterpret_cast<const uint4*>(x + (size_t)r0 * ld);
+    if (page == -2) page = kv_page(p, w);
+    if (page < 0) return;
+    const size_t line = (size_t)page * p.kv_heads + head;
+    int8_t* codes = (val ? p.v : p.k) + line * (size_t)(kPage * D);
+    uint16_t* scale = (val ? p.vs : p.ks) + line;
+    const uint32_t was = *scale;
+    uint32_t most = max_bits(first);
+    for (int r = r0 + kRowsAt; r < w.count; r += kRowsAt)
+      most = __vmaxu2(most, max_bits(*reinterpret_cast<const uint4*>(x + (size_t)r * ld)));
+    most = max(most & 0xffffu, most >> 16);
+    most = __reduce_max_sync(0xffffffffu, most);
+    const uint32_t now = joined_scale(most, was, w.from > 0);
+    if (w.from > 0 && now != was && now <= 0x7f7fu)
+      rescale_codes(codes, w.from * (D / 4), was, now, lane, 32);
+    __syncwarp();                                      // all have read `was`
+    if (lane == 0 && (w.from == 0 || now != was)) *scale = (uint16_t)now;
+    const KvCoder coder(now);
+    for (int r = r0; r < w.count; r += kRowsAt) {
+      const uint4 in = r == r0 ? first : *reinterpret_cast<const uint4*>(x + (size_t)r * ld);
+      *reinterpret_cast<uint2*>(codes + (size_t)(w.from + r) * D + chunk * 8) =
+          now > 0x7f7fu ? make_uint2(0, 0) : coder.eight(in);
+    }
   }
 }
 
@@ -188,28 +293,40 @@ template <int D>
 __global__ void __launch_bounds__(kAppendThreads)
     kv8_read_kernel(KvPages p, __nv_bfloat16* k, int ldk, __nv_bfloat16* v, int ldv)
 {
-  constexpr int kChunks = D / 16;
+  constexpr int kChunks = D / 16, kMost = kPage * kChunks / kAppendThreads;
   pdl_wait();
   pdl_trigger();
-  KvSpan w;
-  if (!kv_span(p, (int)blockIdx.x, (int)blockIdx.y, &w)) return;
+  const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+  const KvSpan w = kv_span(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
+  if (w.count == 0) return;
+  const int page = kv_page(p, w);
+  if (page < 0) return;
   const bool val = blockIdx.z != 0;
   __nv_bfloat16* x = val ? v : k;
   const int ld = val ? ldv : ldk;
-  const int8_t* codes = (val ? p.v : p.k) + w.page * (size_t)(kPage * D) + (size_t)w.from * D;
-  const float s = bf16_bits((val ? p.vs : p.ks)[w.page]);
-  for (int i = (int)threadIdx.x; i < w.count * kChunks; i += kAppendThreads) {
-    const uint4 c = reinterpret_cast<const uint4*>(codes)[i];
-    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+  const size_t line = (size_t)page * p.kv_heads + head;
+  const int8_t* codes = (val ? p.v : p.k) + line * (size_t)(kPage * D) + (size_t)w.from * D;
+  const float s = bf16_bits((val ? p.vs : p.ks)[line]);
+  uint4 c[kMost];
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int i = (int)threadIdx.x + j * kAppendThreads;
+    if (i < w.count * kChunks) c[j] = reinterpret_cast<const uint4*>(codes)[i];
+  }
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int i = (int)threadIdx.x + j * kAppendThreads;
+    if (i >= w.count * kChunks) break;
+    const uint32_t words[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
     uint32_t o[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const char4 b = *reinterpret_cast<const char4*>(&words[j]);
-      o[2 * j] = pack_bf16((float)b.x * s, (float)b.y * s);
-      o[2 * j + 1] = pack_bf16((float)b.z * s, (float)b.w * s);
+    for (int e = 0; e < 4; ++e) {
+      const char4 b = *reinterpret_cast<const char4*>(&words[e]);
+      o[2 * e] = pack_bf16((float)b.x * s, (float)b.y * s);
+      o[2 * e + 1] = pack_bf16((float)b.z * s, (float)b.w * s);
     }
     uint4* dst = reinterpret_cast<uint4*>(x + (size_t)(w.row + i / kChunks) * ld +
-                                          (size_t)blockIdx.y * D + (i % kChunks) * 16);
+                                          (size_t)head * D + (i % kChunks) * 16);
     dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
     dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
@@ -1126,9 +1243,13 @@ KvPages kv_pages(const Kv8Cache& c, const Kv8Rows& r, int* err)
   return p;
 }
 
-dim3 kv_pages_grid(const Kv8Cache& c, const Kv8Rows& r)
+// blocks of a page and head, keys and values
+bool kv_pages_grid(const Kv8Cache& c, const Kv8Rows& r, dim3* grid)
 {
-  return dim3((unsigned)slot_count(r.rows, r.seqs, kPage, 2), (unsigned)c.kv_heads, 2);
+  const long long n = (long long)slot_count(r.rows, r.seqs, kPage, 2) * c.kv_heads;
+  if (n > INT_MAX) return false;
+  *grid = dim3((unsigned)n, 1, 2);
+  return true;
 }
 
 template <int D, int NR>
@@ -1197,11 +1318,25 @@ int launch_kv8_append(const Kv8Cache& c, const Kv8Rows& r, const __nv_bfloat16* 
                       const __nv_bfloat16* v, int ldv, int* err, cudaStream_t s)
 {
   const KvPages p = kv_pages(c, r, err);
-  const dim3 grid = kv_pages_grid(c, r);
+  // few rows a sequence: a block a page; else one for each of its heads, keys and values
+  const bool few = (long long)r.rows <= 4ll * r.seqs;
+  dim3 grid;
+  if (few) grid = dim3((unsigned)slot_count(r.rows, r.seqs, kPage, 2));
+  else if (!kv_pages_grid(c, r, &grid)) return -2;
+  const dim3 block(kAppendThreads);
   switch (c.head_dim) {
-    case 64: launch_k(kv8_append_kernel<64>, grid, dim3(kAppendThreads), 0, s, 1, p, k, ldk, v, ldv); break;
-    case 128: launch_k(kv8_append_kernel<128>, grid, dim3(kAppendThreads), 0, s, 1, p, k, ldk, v, ldv); break;
-    case 256: launch_k(kv8_append_kernel<256>, grid, dim3(kAppendThreads), 0, s, 1, p, k, ldk, v, ldv); break;
+    case 64:
+      launch_k(few ? kv8_append_few_kernel<64> : kv8_append_kernel<64>, grid, block, 0, s, 1, p, k,
+               ldk, v, ldv);
+      break;
+    case 128:
+      launch_k(few ? kv8_append_few_kernel<128> : kv8_append_kernel<128>, grid, block, 0, s, 1, p,
+               k, ldk, v, ldv);
+      break;
+    case 256:
+      launch_k(few ? kv8_append_few_kernel<256> : kv8_append_kernel<256>, grid, block, 0, s, 1, p,
+               k, ldk, v, ldv);
+      break;
     default: return -2;
   }
   return launched();
@@ -1211,7 +1346,8 @@ int launch_kv8_read(const Kv8Cache& c, const Kv8Rows& r, __nv_bfloat16* k, int l
                     __nv_bfloat16* v, int ldv, int* err, cudaStream_t s)
 {
   const KvPages p = kv_pages(c, r, err);
-  const dim3 grid = kv_pages_grid(c, r);
+  dim3 grid;
+  if (!kv_pages_grid(c, r, &grid)) return -2;
   switch (c.head_dim) {
     case 64: launch_k(kv8_read_kernel<64>, grid, dim3(kAppendThreads), 0, s, 1, p, k, ldk, v, ldv); break;
     case 128: launch_k(kv8_read_kernel<128>, grid, dim3(kAppendThreads), 0, s, 1, p, k, ldk, v, ldv); break;
