@@ -1303,13 +1303,18 @@ int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
 }
 
 // Tiles of 8 rows where the sequences have no more on the average (a decoded
-// token under up to 8 query heads a key head), else of 16.
+// token under up to 8 query heads a key head), else of 16 (64 sequences of 100 to
+// 8192 tokens, 16 rows: 142 against 183 us at width 128, 91 against 106 at 64).
+// At width 256 a second group of rows does not fit the registers beside O and q
+// and two tiles are faster (16 sequences, 16 rows, 4096 keys: 88 against 100 us).
 template <int D>
 int kv_attn_tiles(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
 {
-  const long long rows = (long long)a.rows.rows * (a.heads / a.cache.kv_heads);
-  return rows <= 8ll * a.rows.seqs ? kv_attn_launch<D, 1>(a, num_sms, err, s)
-                                   : kv_attn_launch<D, 2>(a, num_sms, err, s);
+  if constexpr (D < 256) {
+    const long long rows = (long long)a.rows.rows * (a.heads / a.cache.kv_heads);
+    if (rows > 8ll * a.rows.seqs) return kv_attn_launch<D, 2>(a, num_sms, err, s);
+  }
+  return kv_attn_launch<D, 1>(a, num_sms, err, s);
 }
 
 }  // namespace
@@ -1359,11 +1364,12 @@ int launch_kv8_read(const Kv8Cache& c, const Kv8Rows& r, __nv_bfloat16* k, int l
 
 size_t kv8_attention_workspace(int head_dim, int num_sms)
 {
-  // the larger of the two tile heights at the width (12 warps x 8 rows at most
-  // beside 8 x 16)
+  // a first and a last part a warp: 12 warps with 8 rows at most, 8 with 16
   const size_t rows = (size_t)num_sms * 2 * 16 * KvCfg<128, 2>::kWarps;
   static_assert(KvCfg<128, 1>::kWarps * 8 <= KvCfg<128, 2>::kWarps * 16 &&
-                KvCfg<256, 2>::kWarps == KvCfg<128, 2>::kWarps, "rows of the workspace");
+                KvCfg<64, 1>::kWarps == KvCfg<128, 1>::kWarps &&
+                KvCfg<64, 2>::kWarps == KvCfg<128, 2>::kWarps &&
+                KvCfg<256, 1>::kWarps <= KvCfg<128, 1>::kWarps, "rows of the workspace");
   return rows * (size_t)(head_dim + 2) * sizeof(float);
 }
 
