@@ -344,17 +344,19 @@ __global__ void __launch_bounds__(kAppendThreads)
 // sum, O) for kv8_merge_kernel.  Measured beside this on 64 ragged sequences
 // and on 32 of one-row tiles (8192 and 4096 tokens at most): runs shared by a
 // block's four warps with a join in shared memory, and parts joined by the last
-// block to arrive, which saves the second launch: 104 and 53 us, half of it
-// waiting at barriers, fences and counters in the middle of a run.
+// block to arrive, which saves the second launch: 104 and 53 us against 91 and 34,
+// the difference spent at barriers, fences and counters in the middle of a run.
 //
 // This reads 2 D bytes a token and key head and is bound by HBM as long as a
 // code costs few instructions.  The products run transposed, S^T = K Q^T and
 // O^T = V^T P^T, on warp MMAs with f32 sums (m16n8k16, f16 operands): 16 keys or
 // 16 output columns by 8 query rows, since a decoded token has no more rows than
 // query heads share a key head.  Against 16 query rows in the M place that halves
-// the MMAs, the exponentials and the registers (measured on 131072 tokens, 8 key
-// heads of 128: 895 to 4xx instructions a stage and warp).  P rounds at 2^-11; q's
-// 8 bits are exact once its row is brought near 2^8 by a power of two.
+// the MMAs, the exponentials and the registers.  P rounds at 2^-11; q's 8 bits are
+// exact once its row is brought near 2^8 by a power of two.  Measured on 131072
+// tokens, 8 key heads of 128 under 4 query heads each: 48.8 us for 268 MB (5.5 TB/s),
+// 739 warp instructions a stage, 55 % of the issue slots, the tensor pipe 19 % busy:
+// bound by what twelve warps of 168 registers keep in flight, then by HBM.
 //   K  byte 128 + c in the low half of an f16 is the subnormal (128 + c) 2^-24:
 //      one byte permute a pair, and 128 sum(q) leaves the score with the
 //      exponent's other constants.
@@ -1088,19 +1090,23 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
 }
 
 // Joins the tiles that several warps share: with M the largest of their
-// maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, in the parts' order.
+// maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, in a fixed order.
 // Writes zeros for the rows of sequences without keys, which no warp has.  A
 // block a (row tile, kv head), or each of its rows where the tiles alone leave SMs
 // idle (grid z); its warps share the rows and, where those are fewer, the parts of
-// a row.  Everything up to pdl_wait reads only what the
-// attention kernel had waited for itself.
+// a row.  It is a chain of latencies (no SM has room for it before the attention
+// ends), so a warp asks for its parts' maxima and their O at once and joins them
+// under its own maximum; the warps of a row join theirs in shared memory (all under
+// the row's maximum, read first: 58.5 against 54.8 us for the case below).
+// Everything up to pdl_wait reads only what the attention kernel had waited for
+// itself.
 template <int D, int NR, int W>
 __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant__ KvAttn p)
 {
-  constexpr int N = 128, E = D / 64, TR = 8 * NR;
+  constexpr int N = 128, E = D / 64, P = E == 4 ? 4 : 8, TR = 8 * NR;
   __shared__ KvTable<N> s_tab;
   __shared__ float2 s_o[W][D / 2];
-  __shared__ float s_l[W];
+  __shared__ float2 s_ml[W];
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   const int head = (int)blockIdx.y, slot = (int)blockIdx.x;
   // the slot's sequence: tiles of rows are slots of cu * group rows
@@ -1130,11 +1136,11 @@ __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant
   u64 at = s_tab.before[s / each];
   for (int i = s / each * each; i < s; ++i) at += kv_work(p, kv_get<D, TR, N>(p, s_tab, i));
   at += ((u64)head * q.tiles + tile) * (u64)q.units;
-  u64 first = 0, last = 0, place0 = 0;
+  int first = 0, last = 0, place0 = 0;                 // workers, the first one's place
   if (rows > r_from && q.units > 0) {
-    first = work_owner(all, workers, at);
-    last = work_owner(all, workers, at + q.units - 1);
-    place0 = work_bound(all, workers, first) < at ? 1 : 0;
+    first = (int)work_owner(all, workers, at);
+    last = (int)work_owner(all, workers, at + q.units - 1);
+    place0 = work_bound(all, workers, (u64)first) < at ? 1 : 0;
   }
   pdl_wait();
   pdl_trigger();
@@ -1148,7 +1154,7 @@ __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant
     return;
   }
   if (first == last) return;                           // written by its warp
-  const int parts = (int)(last - first) + 1;
+  const int parts = last - first + 1;
   auto site = [&](int i, int r) { return ((first + i) * 2 + (i == 0 ? place0 : 0)) * TR + r; };
   // `wide` warps a row, a power of two
   const int own = rows - r_from;
@@ -1156,35 +1162,51 @@ __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant
   for (int r0 = r_from; r0 < rows; r0 += W / wide) {
     const int r = r0 + warp / wide, mine = warp % wide;
     float2 acc[E];
-    float l = 0.0f;
+    float l = 0.0f, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = make_float2(0.0f, 0.0f);
     if (r < rows) {
-      // 32 parts' factors at a time, one a lane; the first batch of each warp has
-      // no maximum to wait for but its own
-      float top = -INFINITY;
-#pragma unroll 4
-      for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[site(i, r) * 2]);
-      for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      const int per = (parts + wide - 1) / wide;       // this warp: parts [mine per, ...)
+      // parts [mine per, end), 32 at a time, a lane each for their factors under the
+      // maximum so far; O of P of them is on its way with the maxima
+      const int per = (parts + wide - 1) / wide;
       const int end = min(parts, (mine + 1) * per);
       for (int i0 = mine * per; i0 < end; i0 += 32) {
-        float f = 0.0f;
-        if (i0 + lane < end) {
-          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + site(i0 + lane, r) * 2);
-          f = kv_weight(ml.x, ml.y, top);
-          l = fmaf(f, ml.y, l);
-        }
         const int n = min(32, end - i0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const float fi = __shfl_sync(0xffffffffu, f, i);
-          const float2* src = reinterpret_cast<const float2*>(p.part_o + site(i0 + i, r) * D) + lane;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + site(i0 + lane, r) * 2);
+        for (int b = 0; b < n; b += P) {
+          float2 v[P][E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float2 v = src[e * 32];
-            acc[e].x = fmaf(fi, v.x, acc[e].x);
-            acc[e].y = fmaf(fi, v.y, acc[e].y);
+          for (int i = 0; i < P; ++i) {
+            const float2* src =
+                reinterpret_cast<const float2*>(p.part_o + (size_t)site(min(i0 + b + i, end - 1), r) * D);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i][e] = src[e * 32 + lane];
+          }
+          if (b == 0) {
+            float most = ml.x;
+            for (int w = 16; w > 0; w >>= 1)
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+            if (most > top) {
+              const float d = top == -INFINITY ? 1.0f : fast_exp2(top - most);
+              l *= d;
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] = make_float2(acc[e].x * d, acc[e].y * d);
+              top = most;
+            }
+            ml.x = kv_weight(ml.x, ml.y, top);
+            l = fmaf(ml.x, ml.y, l);
+          }
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const float f = __shfl_sync(0xffffffffu, ml.x, (b + i) & 31);
+            if (b + i < n) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) {
+                acc[e].x = fmaf(f, v[i][e].x, acc[e].x);
+                acc[e].y = fmaf(f, v[i][e].y, acc[e].y);
+              }
+            }
           }
         }
       }
@@ -1194,19 +1216,30 @@ __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant
       if (r < rows) {
 #pragma unroll
         for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
-        if (lane == 0) s_l[warp] = l;
+        if (lane == 0) s_ml[warp] = make_float2(top, l);
       }
       __syncthreads();
-      if (r < rows && mine == 0)
-        for (int w = 1; w < wide; ++w) {
-          l += s_l[warp + w];
+      if (r < rows && mine == 0) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < wide) ml = s_ml[warp + lane];
+        float most = ml.x;
+        for (int w = 16; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+        const float f = kv_weight(ml.x, ml.y, most);
+        l = f * ml.y;
+        for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+        for (int w = 0; w < wide; ++w) {
+          const float fw = __shfl_sync(0xffffffffu, f, w);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             const float2 v = s_o[warp + w][e * 32 + lane];
-            acc[e].x += v.x;
-            acc[e].y += v.y;
+            acc[e].x = fmaf(fw, v.x, acc[e].x);
+            acc[e].y = fmaf(fw, v.y, acc[e].y);
           }
         }
+      }
     }
     if (r < rows && mine == 0) {
       const int rt = tile * TR + r;
@@ -1289,10 +1322,12 @@ int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
   if (!smem_limit_once(kv8_attention_kernel<D, NR>, C::kSmem, attr)) return -1;
   launch_k(kv8_attention_kernel<D, NR>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1, p);
   if (launched() != 0) return -1;
-  // few tiles have many parts each: 32 warps a row; else a warp a row
+  // few tiles have many parts each: 16 warps a row (1 sequence of 131072 tokens, 222
+  // parts a row: 53.5 us with the attention, 54.8 with 32 warps, 57.1 with 8); else a
+  // warp a row
   if ((long long)slots * p.kv_heads * 2 <= num_sms)
-    launch_k(kv8_merge_kernel<D, NR, 32>, dim3((unsigned)slots, (unsigned)p.kv_heads, 8 * NR),
-             dim3(1024), 0, s, 1, p);
+    launch_k(kv8_merge_kernel<D, NR, 16>, dim3((unsigned)slots, (unsigned)p.kv_heads, 8 * NR),
+             dim3(512), 0, s, 1, p);
   else if ((long long)p.rows * p.group > 4ll * p.seqs)
     launch_k(kv8_merge_kernel<D, NR, 8>, dim3((unsigned)slots, (unsigned)p.kv_heads), dim3(256), 0,
              s, 1, p);
