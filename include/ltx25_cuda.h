@@ -392,7 +392,8 @@ typedef struct {
  * (starts[s] % LTX_KV8_PAGE != 0, first page).  New codes are
  * rint(x / scale); codes the page held are brought to a grown scale as
  * rint(code * old / new).  A NaN or infinity makes the scale of its page and
- * head NaN.  The pages that get tokens belong to one sequence each. */
+ * head NaN.  A page that gets tokens stands once in the table's used columns,
+ * for one sequence. */
 LTX_API int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,
                            const void* v, int ldv, const int32_t* cu, const int32_t* starts,
                            const int32_t* table, int table_ld, int seqs, int rows, void* stream);
@@ -408,7 +409,8 @@ LTX_API int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int 
  * are the last tokens of sequence s, whose lengths[s] tokens (those included)
  * the cache holds; row i of n sees the tokens up to its own position
  * lengths[s] - n + i, with window > 0 only those above position - window.  The
- * result is ltx_attention_packed's over the values the codes stand for.  One
+ * result is ltx_attention_packed's over the values the codes stand for (an
+ * infinity in a row of q makes that row NaN).  o must not overlap q.  One
  * token a sequence is the usual call; the cache is read once for each 16 rows
  * (tokens times the query heads of a key/value head).  max_len sizes the
  * launch: the largest length expected.  The workspace is the caller's,

@@ -144,6 +144,51 @@ def test_what_a_row_does_not_see_does_not_reach_it(ctx, D, value):
     assert torch.equal(seen[~ok].isnan(), ref[~ok].isnan())
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("where", ["k", "v", "both signs in v"])
+def test_what_every_row_sees_reaches_it_alone(ctx, D, where):
+    """A NaN, or infinities of both signs, near the start of a long prefix: NaN where
+    the formula has it, in every row; the other columns and the other key head are
+    what they were."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads, lens_q, lens_k = 4, 2, [200, 40], [9000, 300]
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 13)
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, True, 0, D ** -0.5)
+    bad = torch.zeros_like(want, dtype=torch.bool)
+    if where == "k":
+        k[70, 5] = math.nan
+        bad[:200, :2 * D] = True             # the two query heads of key head 0
+    else:
+        v[70, 5] = math.nan if where == "v" else math.inf
+        if where != "v":
+            v[4000, 5] = -math.inf
+        bad[:200, [5, D + 5]] = True
+    got = L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D)
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.equal(got.isnan(), bad)
+    assert float(((got.double() - want).abs() - tol)[~bad].max()) <= 0
+
+
+def test_calls_beyond_the_kernels_counters_are_refused(ctx):
+    """Before anything is read."""
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu, _ = make([20], [20], 4, 2, 64)
+    c = dev(cu)
+    with pytest.raises(L.LtxError) as e:
+        L.attention_packed(ctx, q, k, v, c, c, 4, 2, 64, scale=3e38)
+    assert e.value.code == -2
+    out = torch.zeros_like(q)
+    rc = ctx.lib.ltx_attention_packed(
+        ctx.h, q.data_ptr(), 256, k.data_ptr(), 256, v.data_ptr(), 256, out.data_ptr(), 256,
+        c.data_ptr(), c.data_ptr(), 2 ** 29 + 1, 20, 20, 4, 2, 64, 1, 0, 0.125, 0)
+    assert rc == -2
+    torch.cuda.synchronize()
+    ctx.check()
+
+
 def test_rows_of_one_projection_and_other_streams(ctx):
     """q, k and v as column slices of one buffer, on a stream of the caller's."""
     import torch

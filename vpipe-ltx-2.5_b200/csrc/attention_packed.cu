@@ -193,26 +193,63 @@ __device__ __forceinline__ void tma_load_3d(const void* map, uint64_t* bar, void
       : "memory");
 }
 
-// Columns [col0, col0 + N) of one output row from the keys [lo, hi) of its
-// sequence alone (rows key0 + j of k and v), in f32, by one warp.
+// The NaNs among columns [col0, col0 + N) of an output row that this warp has
+// stored, looked into: a column with a NaN among its row's own values (rows
+// key0 + j of v, j in [lo, hi)) keeps it; if any is left, the row is computed again
+// from its own keys alone, in f32.  The first pass costs 1/10 of the second, so
+// that a NaN every row sees stays cheap.
 template <int D, int N>
 __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, int kvh, int key0,
                                         int lo, int hi, int col0)
 {
-  constexpr int W = N / 32;                       // dims of a lane
+  constexpr int W = N / 32;                       // columns of a lane, 2 or 4
   const int lane = (int)lane_id();
-  const __nv_bfloat16* q = p.q + (size_t)row * p.ldq + (size_t)head * D;
+  __nv_bfloat16* o = p.o + (size_t)row * p.ldo + (size_t)head * D + col0 + lane * W;
+  const __nv_bfloat16* v0 = p.v + (size_t)key0 * p.ldv + (size_t)kvh * D + col0 + lane * W;
+  bool bad[W], open = false;
+  for (int e = 0; e < W; ++e) {
+    const float x = __bfloat162float(o[e]);
+    bad[e] = x != x;
+    open |= bad[e];
+  }
+  bool found[W] = {};
+  for (int j = lo; j < hi && __any_sync(0xffffffffu, open); j += 16) {
+    open = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __nv_bfloat162* v =
+          reinterpret_cast<const __nv_bfloat162*>(v0 + (size_t)min(j + i, hi - 1) * p.ldv);
+#pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const float2 x = __bfloat1622float2(v[e / 2]);
+        found[e] |= x.x != x.x;
+        found[e + 1] |= x.y != x.y;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) open |= bad[e] && !found[e];
+  }
+  if (!__any_sync(0xffffffffu, open)) return;
+
+  const uint4* q = reinterpret_cast<const uint4*>(p.q + (size_t)row * p.ldq + (size_t)head * D);
   float m = -INFINITY, l = 0.0f, acc[W];
   for (int e = 0; e < W; ++e) acc[e] = 0.0f;
   for (int j0 = lo; j0 < hi; j0 += 32) {
     const int n = min(32, hi - j0);
-    float s = -INFINITY;
-    if (lane < n) {
-      const __nv_bfloat16* k = p.k + (size_t)(key0 + j0 + lane) * p.ldk + (size_t)kvh * D;
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), dot);
-      s = dot * p.c;
+    const uint4* k = reinterpret_cast<const uint4*>(
+        p.k + (size_t)(key0 + j0 + min(lane, n - 1)) * p.ldk + (size_t)kvh * D);
+    float dot = 0.0f;
+#pragma unroll 4
+    for (int d = 0; d < D / 8; ++d) {
+      const uint4 a = q[d], b = k[d];
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dot = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), dot);
+        dot = fmaf(__uint_as_float(aw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), dot);
+      }
     }
+    const float s = lane < n ? dot * p.c : -INFINITY;
     float mx = s;
     for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
     const float m_new = fmaxf(m, mx);
@@ -222,15 +259,22 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
     m = m_new;
     l = l * f + pj;                               // this lane's share
     for (int e = 0; e < W; ++e) acc[e] *= f;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const float pi = __shfl_sync(0xffffffffu, pj, i);
-      const __nv_bfloat16* v = p.v + (size_t)(key0 + j0 + i) * p.ldv + (size_t)kvh * D + col0;
-      for (int e = 0; e < W; ++e) acc[e] = fmaf(pi, __bfloat162float(v[lane * W + e]), acc[e]);
+      const __nv_bfloat162* v =
+          reinterpret_cast<const __nv_bfloat162*>(v0 + (size_t)(j0 + i) * p.ldv);
+#pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const float2 x = __bfloat1622float2(v[e / 2]);
+        acc[e] = fmaf(pi, x.x, acc[e]);
+        acc[e + 1] = fmaf(pi, x.y, acc[e + 1]);
+      }
     }
   }
   for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-  __nv_bfloat16* o = p.o + (size_t)row * p.ldo + (size_t)head * D + col0;
-  for (int e = 0; e < W; ++e) o[lane * W + e] = __float2bfloat16_rn(acc[e] / l);
+  for (int e = 0; e < W; ++e)
+    if (bad[e]) o[e] = __float2bfloat16_rn(acc[e] / l);
 }
 
 // Bits [from, to) of 32, both bounds anywhere.
@@ -908,11 +952,13 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         const bool valid_row = r < p.tq * p.group && tok < w->nq;
         const int row = w->row0 + tok, head = w->head * p.group + r % p.group;
         const float g = 1.0f / l_row;
+        // a sum of 0 or NaN is of the row's own keys and makes all of it NaN
+        const bool fix = valid_row && l_row > 0.0f;
         const long long to = (long long)row * p.ldo + (long long)head * D + hh * kCols;
         const bool nan = store_row<kCols>(orow + (uint32_t)(hh * kCols), nt > 0, sees, g, p.o,
                                           valid_row ? to : -1, &o_free[t]);
         __syncwarp();                                  // repair_row follows on these stores
-        uint32_t bad = __ballot_sync(0xffffffffu, nan && valid_row);
+        uint32_t bad = __ballot_sync(0xffffffffu, nan && fix);
         while (bad != 0) {
           const int src = __ffs((int)bad) - 1;
           bad &= bad - 1;

@@ -11,6 +11,9 @@ namespace ltx25 {
 
 namespace {
 
+// Work slots are counted in 32 bits, up to two a sequence beside those of its rows.
+constexpr int kMaxSeqs = 1 << 29;
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // heads, head width and the factor of the scores
@@ -30,8 +33,9 @@ int check_heads(const char* op, int heads, int kv_heads, int head_dim, int windo
     *why = o + ": need window >= 0 (0: no window)";
     return LTX_E_SHAPE;
   }
-  if (!(scale > 0.0f) || !std::isfinite(scale)) {
-    *why = o + ": need a finite scale > 0";
+  // the kernels take it times log2 e
+  if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f)) {
+    *why = o + ": need a scale > 0, below 2e38";
     return LTX_E_SHAPE;
   }
   return LTX_OK;
@@ -81,7 +85,7 @@ int check_cache(const char* op, const ltx::Kv8Cache& c, const ltx::Kv8Rows& r, s
     *why = o + ": need pages >= 0, kv_heads 1..65535, head_dim 64, 128 or 256";
     return LTX_E_SHAPE;
   }
-  if (r.seqs < 0 || r.rows < 0 || r.seqs > (1 << 29) || r.table_ld < 1 || r.table_ld > (1 << 24)) {
+  if (r.seqs < 0 || r.rows < 0 || r.seqs > kMaxSeqs || r.table_ld < 1 || r.table_ld > (1 << 24)) {
     *why = o + ": need seqs 0..2^29, rows >= 0, table columns 1..2^24";
     return LTX_E_SHAPE;
   }
@@ -148,8 +152,8 @@ int check_attention_packed(const ltx::PackedAttention& a, std::string* why)
   const char* op = "attention_packed";
   int rc = check_heads(op, a.heads, a.kv_heads, a.head_dim, a.window, a.scale, why);
   if (rc != LTX_OK) return rc;
-  if (a.seqs < 0 || a.rows < 0 || a.keys < 0) {
-    *why = "attention_packed: need seqs, rows and keys >= 0";
+  if (a.seqs < 0 || a.rows < 0 || a.keys < 0 || a.seqs > kMaxSeqs) {
+    *why = "attention_packed: need seqs 0..2^29, rows and keys >= 0";
     return LTX_E_SHAPE;
   }
   if (a.seqs == 0 || a.rows == 0) return LTX_OK;
