@@ -240,6 +240,27 @@ def test_attention_over_far_apart_scales(ctx, D, qscale, spread):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("a,b", [(116, 100), (-90, -100), (100, 0)])
+def test_attention_under_powers_of_two(ctx, D, a, b):
+    """q by 2^a against K's scales by 2^-a, V's scales by 2^b: the products are the
+    same and o is 2^b times as large.  Both are within f32's error of the same number,
+    so they round to neighbours at most: a step of 2^-7."""
+    import torch
+    import ltx25_b200 as L
+    new, lengths, heads, kv_heads = [1, 3], [900, 70], 4, 2
+    cache, q, cu, table = attention_case(ctx, new, lengths, heads, kv_heads, D, 0)
+    far = L.KV8Cache(cache.k, cache.v, (cache.k_scale.double() * 2.0 ** -a).to(torch.bfloat16),
+                     (cache.v_scale.double() * 2.0 ** b).to(torch.bfloat16))
+    args = (ints(cu), ints(lengths), ints(table), heads, 900)
+    near = L.kv8_attention(ctx, cache, q, *args).double()
+    got = L.kv8_attention(ctx, far, (q.double() * 2.0 ** a).to(torch.bfloat16), *args).double()
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.isfinite(got).all()
+    assert bool(((got * 2.0 ** -b - near).abs() <= near.abs() * 2.0 ** -7).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_attention_does_not_look_past_a_row_s_tokens(ctx, D):
     """Scales of NaN on pages past the end, before the window, and on the page of a
     later new token; codes behind the last token of a page."""
@@ -407,6 +428,19 @@ def test_places_outside_the_cache_are_not_followed(ctx):
         L.kv8_attention(ctx, cache, rows_of(10, heads * D, 2), ints(cu), ints([100]),
                         ints(table[:1]), heads, 256)
         torch.cuda.synchronize()
+    ctx.check()
+
+
+def test_a_scale_that_leaves_32_bits_is_refused(ctx):
+    import torch
+    import ltx25_b200 as L
+    table, pages = tables([2])
+    cache = cache_of(pages, 2, 64)
+    args = (ints([0, 1]), ints([5]), ints(table), 4, 64)
+    with pytest.raises(L.LtxError) as e:
+        L.kv8_attention(ctx, cache, rows_of(1, 256, 2), *args, scale=3e38)
+    assert e.value.code == -2
+    torch.cuda.synchronize()
     ctx.check()
 
 

@@ -777,7 +777,8 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
       if (most == 0 || most > 0x7f7fu) ex = 8;
       ex = max(ex, -100);
       const float up = __uint_as_float((uint32_t)(127 + 8 - ex) << 23);
-      const float factor = p.c * 16777216.0f * __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
+      // (2^24 of K's codes comes in with K's scale, so that this stays finite)
+      const float factor = p.c * __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < D / 64; ++j)
@@ -926,7 +927,7 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
           float fo[2] = {turn, turn};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            f[e] = qs[h][e] * ks;
+            f[e] = qs[h][e] * ks * 16777216.0f;
             float mx = fmaxf(s[0][e], s[0][2 + e]);
 #pragma unroll
             for (int t = 1; t < MT; ++t) mx = max3f(mx, s[t][e], s[t][2 + e]);
