@@ -189,6 +189,30 @@ def test_calls_beyond_the_kernels_counters_are_refused(ctx):
     ctx.check()
 
 
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 8, 8), (128, 32, 4), (256, 12, 6)])
+@pytest.mark.parametrize("causal,window,prefix", [(True, 0, 0), (True, 200, 0), (True, 0, 90),
+                                                  (False, 0, 0), (False, 70, 33)])
+@pytest.mark.parametrize("seqs", [2, 17, 32, 33])
+def test_more_items_than_sms(ctx, D, heads, kv_heads, causal, window, prefix, seqs):
+    """Items that wait for a place, of sequences of 0 to 1100 tokens: each is done, and
+    done once, in whatever order; some sequences have no keys, some more rows than keys."""
+    import random
+    import torch
+    import ltx25_b200 as L
+    rng = random.Random(seqs * D + window)
+    lens_q = [rng.choice([0, 1, rng.randint(2, 300), rng.randint(300, 1100)]) for _ in range(seqs)]
+    lens_q[0] = 1100
+    lens_k = [max(0, n + rng.choice([prefix, 0, -n, -5])) for n in lens_q]
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 21)
+    got = L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D, causal=causal,
+                             window=window)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, causal, window,
+                                        D ** -0.5)
+    check(got, want, tol, cu_q)
+
+
 def test_rows_of_one_projection_and_other_streams(ctx):
     """q, k and v as column slices of one buffer, on a stream of the caller's."""
     import torch

@@ -27,6 +27,9 @@ unsigned long long t_bound(unsigned long long a, unsigned long long w, unsigned 
 { return ltx::work_bound(a, w, i); }
 unsigned long long t_owner(unsigned long long a, unsigned long long w, unsigned long long x)
 { return ltx::work_owner(a, w, x); }
+int t_top(int n, int m, int t, int c, int w) { return ltx::top_level(ltx::tile_levels(n, m, t, c, w)); }
+int t_above(int n, int m, int t, int c, int w, int l)
+{ return ltx::tiles_above(ltx::tile_levels(n, m, t, c, w), l); }
 int t_clamp(int v, int lo, int hi) { return ltx::clamp_int(v, lo, hi); }
 }
 """
@@ -135,3 +138,35 @@ def test_equal_runs_of_work(idx):
     big = 1 << 40                                       # beyond 32 bits
     assert idx.t_owner(u(big), u(1184), u(big - 1)) == 1183
     assert idx.t_bound(u(big), u(1184), u(1184)) == big
+
+
+def test_tiles_come_in_order_of_their_keys(idx):
+    """tiles_above is the number of tiles whose level is higher, all of them at -1, none
+    at the top; a causal sequence's are its last ones."""
+    rng = random.Random(5)
+    big = 2 ** 31 - 1
+    for i in range(3000):
+        t = rng.choice([1, 4, 25, 64, 128, 512])
+        n, m = rng.choice([0, 1, t, rng.randint(0, 9 * t)]), rng.randint(0, 12 * t)
+        window = rng.choice([0, 0, 1, t, 3 * t + 5, big])
+        causal = rng.randint(0, 1)
+        tiles = -(-n // t)
+        cap = big if window == 0 else min(big, (window + t) // t + 1)
+        level = []
+        for k in range(tiles):
+            reach = m - n + (k + 1) * t if causal else m
+            level.append(min(cap, max(0, -(-reach // t))))
+        assert level == sorted(level)
+        top = idx.t_top(n, m, t, causal, window)
+        assert top == max(level + [0])
+        for lv in range(-1, top + 2):
+            assert idx.t_above(n, m, t, causal, window, lv) == sum(x > lv for x in level)
+    # the largest sizes stay in range
+    for n, m, t in ((big, big, 1), (big, 0, 1), (0, big, 1), (big, big, 512), (1, big, 4)):
+        for causal in (0, 1):
+            tiles = -(-n // t)
+            top = idx.t_top(n, m, t, causal, 0)
+            assert 0 <= top and idx.t_above(n, m, t, causal, 0, top) == 0
+            assert idx.t_above(n, m, t, causal, 0, -1) == tiles
+            assert all(0 <= idx.t_above(n, m, t, causal, 0, lv) <= tiles
+                       for lv in (0, 1, top // 2, max(0, top - 1)))

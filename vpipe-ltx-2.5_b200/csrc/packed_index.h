@@ -44,6 +44,47 @@ LTX_HD int key_low(int pos, int window)
   return window > 0 && pos >= window ? pos - window + 1 : 0;
 }
 
+// The query tiles of a sequence, `t` rows each, by how far their keys reach: tile i
+// is of level ceil(reach / t), where reach is the m keys, or causal those up to its
+// last row's position, m - n + (i + 1) t, and `cap` at most (a window's).  Levels are
+// for ordering alone; the last tile counts as a whole one.
+struct TileLevels {
+  int tiles, t, cap, whole;       // whole: all tiles reach all of m
+  long long shift;                // m - n, or m
+};
+LTX_HD TileLevels tile_levels(int n, int m, int t, int causal, int window)
+{
+  TileLevels l;
+  l.tiles = (int)(((unsigned)n + (unsigned)t - 1u) / (unsigned)t);
+  l.t = t;
+  l.cap = 0x7fffffff;
+  if (window > 0) {
+    const unsigned cap = ((unsigned)window + (unsigned)t) / (unsigned)t + 1u;
+    if (cap < 0x7fffffffu) l.cap = (int)cap;
+  }
+  l.whole = !causal;
+  l.shift = causal ? (long long)m - n : m;
+  return l;
+}
+// The largest level; the number of tiles above a level (-1: all).
+LTX_HD int top_level(const TileLevels& l)
+{
+  if (l.tiles == 0) return 0;
+  const long long reach = l.shift + (l.whole ? 0 : (long long)l.tiles * l.t);
+  if (reach <= 0) return 0;
+  const unsigned top = ((unsigned)reach + (unsigned)l.t - 1u) / (unsigned)l.t;   // reach <= m + t
+  return top < (unsigned)l.cap ? (int)top : l.cap;
+}
+LTX_HD int tiles_above(const TileLevels& l, int level)
+{
+  if (level < 0) return l.tiles;
+  if (level >= l.cap) return 0;
+  const long long most = (long long)level * l.t - l.shift;  // tile i is above: (i + 1) t > most
+  if (l.whole) return most < 0 ? l.tiles : 0;
+  if (most >= (long long)l.tiles * l.t) return 0;
+  return l.tiles - (most < 0 ? 0 : (int)((unsigned)most / (unsigned)l.t));
+}
+
 // ---- the paged cache -------------------------------------------------------
 
 constexpr int kPage = 64;         // tokens of a page
