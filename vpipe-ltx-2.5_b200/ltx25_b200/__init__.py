@@ -799,19 +799,22 @@ def _rows(ctx, t, cols, name, rows=None):
     """The row stride of a [rows][cols] bf16 tensor on the context's device with
     adjacent columns."""
     import torch
+    shape = t.shape
     if t.dtype is not torch.bfloat16:
         raise LtxError(-3, f"{name}: need bfloat16, got {t.dtype}")
-    shape = t.shape
-    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+    if len(shape) != 2:
+        raise LtxError(-2, f"{name}: need two dimensions, got {tuple(shape)}")
+    n, c = shape
+    if c != cols or (rows is not None and n != rows):
         raise LtxError(-2, f"{name}: need [{'rows' if rows is None else rows}][{cols}], got "
                            f"{tuple(shape)}")
     if t.get_device() != ctx.device:
         raise _elsewhere(ctx, t, name)
-    if shape[0] < 2:                     # one row (or none) has no stride to speak of
-        if shape[0] == 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if n < 2:                            # one row (or none) has no stride to speak of
+        if n == 1 and one != 1:
             raise LtxError(-2, f"{name}: need adjacent columns")
         return (cols + 7) // 8 * 8
-    ld, one = t.stride()
     if one != 1 or ld < cols:            # broadcast rows too
         raise LtxError(-2, f"{name}: need adjacent columns and rows that do not overlap, got "
                            f"strides {t.stride()}")
@@ -821,23 +824,22 @@ def _rows(ctx, t, cols, name, rows=None):
 def _ints(ctx, t, n, name):
     """The address of n adjacent int32 values on the context's device."""
     import torch
-    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
-        raise LtxError(-2, f"{name}: need {n} adjacent int32 values, got {tuple(t.shape)} "
-                           f"{t.dtype}")
+    if t.dtype is torch.int32 and t.numel() == n and t.get_device() == ctx.device and \
+            t.is_contiguous():
+        return t.data_ptr()
     if t.get_device() != ctx.device:
         raise _elsewhere(ctx, t, name)
-    return t.data_ptr()
+    raise LtxError(-2, f"{name}: need {n} adjacent int32 values, got {tuple(t.shape)} {t.dtype}")
 
 
 def _table(ctx, t, seqs):
     """The address and columns of a page table, int32 [seqs][columns]."""
     import torch
-    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != seqs or not t.is_contiguous():
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != seqs:
         raise LtxError(-2, f"table: need contiguous int32 [{seqs}][columns], got "
-                           f"{tuple(t.shape)} {t.dtype}")
-    if t.get_device() != ctx.device:
-        raise _elsewhere(ctx, t, "table")
-    return t.data_ptr(), t.shape[1]
+                           f"{tuple(shape)} {t.dtype}")
+    return _ints(ctx, t, t.numel(), "table"), shape[1]
 
 
 def attention_packed(ctx, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal=True, window=0,
