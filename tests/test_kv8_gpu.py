@@ -239,6 +239,26 @@ def test_attention_over_far_apart_scales(ctx, D, qscale, spread):
     close(got, want, tol)
 
 
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 3, 3), (64, 16, 1), (128, 8, 2), (128, 40, 4),
+                                              (256, 4, 2), (256, 9, 1)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_of_short_sequences(ctx, D, heads, kv_heads, window):
+    """Lengths from nothing to a few stages a warp, one new token each or several or
+    none, more new tokens than the sequence holds; the same with room for long ones."""
+    import torch
+    import ltx25_b200 as L
+    lengths = [0, 1, 15, 16, 17, 63, 64, 65, 191, 400, 900, 2]
+    for new in ([1] * 12, [1, 1, 2, 0, 5, 3, 0, 1, 4, 1, 2, 9]):
+        cache, q, cu, table = attention_case(ctx, new, lengths, heads, kv_heads, D, window)
+        want, tol = expect(cache, q, cu, lengths, table, heads, window)
+        for max_len in (900, 100000):
+            got = L.kv8_attention(ctx, cache, q, ints(cu), ints(lengths), ints(table), heads,
+                                  max_len, window=window)
+            torch.cuda.synchronize()
+            ctx.check()
+            close(got, want, tol)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("a,b", [(116, 100), (-90, -100), (100, 0)])
 def test_attention_under_powers_of_two(ctx, D, a, b):

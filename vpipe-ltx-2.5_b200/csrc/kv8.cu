@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kAppendThreads)
 // block's four warps with a join in shared memory, and parts joined by the last
 // block to arrive, which saves the second launch: 104 and 53 us against 91 and 34,
 // the difference spent at barriers, fences and counters in the middle of a run.
+// Few short tiles are a block's each instead, in one launch (kv_attn_launch).
 //
 // This reads 2 D bytes a token and key head and is bound by HBM as long as a
 // code costs few instructions.  The products run transposed, S^T = K Q^T and
@@ -372,8 +373,9 @@ __global__ void __launch_bounds__(kAppendThreads)
 // the MMAs, the exponentials and the registers.  P rounds at 2^-11; q's 8 bits are
 // exact once its row is brought near 2^8 by a power of two.  Measured on 131072
 // tokens, 8 key heads of 128 under 4 query heads each: 48.8 us for 268 MB (5.5 TB/s),
-// 739 warp instructions a stage, 55 % of the issue slots, the tensor pipe 19 % busy:
-// bound by what twelve warps of 168 registers keep in flight, then by HBM.
+// 739 warp instructions a stage (903 that way), 55 % of the issue slots, tensor pipe
+// 19 %.  5 us of it are the start (offsets, pages, then keys wait for one another); the
+// rest is HBM at 6.1 TB/s.
 //   K  byte 128 + c in the low half of an f16 is the subnormal (128 + c) 2^-24:
 //      one byte permute a pair, and 128 sum(q) leaves the score with the
 //      exponent's other constants.
@@ -642,8 +644,25 @@ __device__ __forceinline__ float kv_weight(float m, float l, float top)
   return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - top);
 }
 
-// NR: groups of 8 query rows of a tile.
-template <int D, int NR>
+// One row of a tile out of f32: columns 2 (32 e + lane) and the next of this lane.
+template <int D>
+__device__ __forceinline__ void kv_put_row(const KvAttn& p, const KvSeq& q, int head, int rt,
+                                           const float2 (&acc)[D / 64], float l)
+{
+  const int tok = rt / p.group, pos = q.len - q.n + tok, lane = (int)lane_id();
+  const bool sees = key_high(pos, q.len, 1) > key_low(pos, p.window);
+  const float norm = 1.0f / l;
+  __nv_bfloat16* dst = p.o + (size_t)(q.row0 + tok) * p.ldo +
+                       (size_t)(head * p.group + rt % p.group) * D;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+    *reinterpret_cast<uint32_t*>(dst + (e * 32 + lane) * 2) =
+        sees ? pack_bf16(acc[e].x * norm, acc[e].y * norm) : 0u;
+}
+
+// NR: groups of 8 query rows of a tile.  TEAM: a block has a tile and its warps
+// share the stages, joined in shared memory; no second launch, no workspace.
+template <int D, int NR, bool TEAM>
 __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
     kv8_attention_kernel(const __grid_constant__ KvAttn p)
 {
@@ -651,6 +670,8 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
   constexpr int T = C::kTok, W = C::kWarps, N = C::kThreads, TR = 8 * NR, MT = C::kMT, OT = C::kOT;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ KvTable<N> s_tab;
+  __shared__ __align__(8) float s_ml[TEAM ? W : 1][TEAM ? TR : 1][2];
+  static_assert(TR * D * 4 <= 2 * C::kStageBytes && W <= 32, "a part takes the place of the stages");
   const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   const int g = lane >> 2, cc = lane & 3;
   uint8_t* const mine = smem_raw + warp * 2 * C::kStageBytes;
@@ -667,15 +688,42 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // this warp's run of the work; neighbours in it are on different SMs
   kv_scan<D, TR, N>(p, s_tab);
-  const u64 all = s_tab.before[N];
-  const u64 workers = kv_workers(p, all);
-  const u64 me = (u64)warp * gridDim.x + blockIdx.x;
-  if (me >= workers) return;
-  const u64 begin = work_bound(all, workers, me);
-  const uint32_t count = (uint32_t)(work_bound(all, workers, me + 1) - begin);
-  KvPlace at = kv_locate<D, TR, N>(p, s_tab, begin);
+  KvPlace at;
+  uint32_t count;
+  size_t site = 0;                                     // of this warp's parts
+  int team = 0;
+  if constexpr (TEAM) {
+    const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads);
+    int hi = p.seqs;                                   // N at most
+    at.s = 0;
+    while (hi - at.s > 1) {
+      const int mid = (at.s + hi) / 2;
+      if (slot_base(s_tab.q[mid].row0 * p.group, mid, TR, 1) <= slot) at.s = mid;
+      else hi = mid;
+    }
+    at.q = s_tab.q[at.s];
+    at.head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    at.tile = slot - slot_base(at.q.row0 * p.group, at.s, TR, 1);
+    if (at.tile < 0 || at.tile >= at.q.tiles) return;  // the whole block
+    team = min(W, at.q.units);                         // warps with a part
+    at.unit = 0;
+    count = 0;
+    if (warp < team) {
+      at.unit = (int)work_bound((u64)at.q.units, (u64)team, (u64)warp);
+      count = (uint32_t)((int)work_bound((u64)at.q.units, (u64)team, (u64)warp + 1) - at.unit);
+    }
+  } else {
+    // this warp's run of the work; neighbours in it are on different SMs
+    const u64 all = s_tab.before[N];
+    const u64 workers = kv_workers(p, all);
+    const u64 me = (u64)warp * gridDim.x + blockIdx.x;
+    if (me >= workers) return;
+    const u64 begin = work_bound(all, workers, me);
+    count = (uint32_t)(work_bound(all, workers, me + 1) - begin);
+    at = kv_locate<D, TR, N>(p, s_tab, begin);
+    site = me * 2 * TR;
+  }
 
   // The loading side: the next stage, and the pages of 32 blocks of its
   // sequence, one a lane.  Scales arrive in registers two stages ahead of their
@@ -1059,9 +1107,16 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
     }
 
     // ---- the tile's rows, or this share's part of them
-    const bool whole = at.unit == 0 && share == (uint32_t)at.q.units;
-    // a warp's first tile goes to place 0, another to 1
-    const size_t site = (me * 2 + (x == 0 ? 0 : 1)) * TR;
+    const bool whole = !TEAM && at.unit == 0 && share == (uint32_t)at.q.units;
+    // a warp's first tile goes to place 0, another to 1; TEAM: over the stages, which
+    // all lanes have read
+    float* part_o = p.part_o + site * D;
+    float* part_ml = p.part_ml + site * 2;
+    if constexpr (TEAM) {
+      part_o = reinterpret_cast<float*>(mine);
+      part_ml = s_ml[warp][0];
+      __syncwarp();
+    }
     const float unit = ref > 0.0f ? ref : 1.0f;
 #pragma unroll
     for (int h = 0; h < NR; ++h)
@@ -1090,21 +1145,53 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float* dst = p.part_o + (site + r) * D;
+          float* dst = part_o + r * D;
 #pragma unroll
           for (int t = 0; t < OT; t += 2)
             *reinterpret_cast<float4*>(dst + t / J * 128 + g * 2 * J + t % J * 2) =
                 make_float4(o[h][t][e] * unit, o[h][t][2 + e] * unit, o[h][t + 1][e] * unit,
                             o[h][t + 1][2 + e] * unit);
           if (g == 0)
-            *reinterpret_cast<float2*>(p.part_ml + (site + r) * 2) =
-                make_float2(m[h][e], l[h][e]);
+            *reinterpret_cast<float2*>(part_ml + r * 2) = make_float2(m[h][e], l[h][e]);
         }
       }
     x += share;
-    if (x < count) kv_move<D, TR, N>(p, s_tab, at, (int)share);
+    if (!TEAM && x < count) {
+      if (x == share) site += TR;
+      kv_move<D, TR, N>(p, s_tab, at, (int)share);
+    }
   }
   cp_async_wait<0>();
+
+  if constexpr (TEAM) {
+    __syncthreads();
+    const int rows = min(TR, at.q.n * p.group - at.tile * TR);
+    for (int r = warp; r < rows; r += W) {
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (lane < team) ml = *reinterpret_cast<const float2*>(s_ml[lane][r]);
+      float top = ml.x;
+      for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float f = kv_weight(ml.x, ml.y, top);
+      float sum = f * ml.y;
+      for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      float2 acc[D / 64];
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) acc[e] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+      for (int w = 0; w < team; ++w) {
+        const float fw = __shfl_sync(0xffffffffu, f, w);
+        const float2* src =
+            reinterpret_cast<const float2*>(smem_raw + w * 2 * C::kStageBytes) + r * (D / 2);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+          const float2 v = src[e * 32 + lane];
+          acc[e].x = fmaf(fw, v.x, acc[e].x);
+          acc[e].y = fmaf(fw, v.y, acc[e].y);
+        }
+      }
+      kv_put_row<D>(p, at.q, at.head, at.tile * TR + r, acc, sum);
+    }
+  }
 }
 
 // Joins the tiles that several warps share: with M the largest of their
@@ -1259,18 +1346,7 @@ __global__ void __launch_bounds__(W * 32) kv8_merge_kernel(const __grid_constant
         }
       }
     }
-    if (r < rows && mine == 0) {
-      const int rt = tile * TR + r;
-      const int tok = rt / p.group, pos = q.len - q.n + tok;
-      const bool sees = key_high(pos, q.len, 1) > key_low(pos, p.window);
-      const float norm = 1.0f / l;
-      __nv_bfloat16* dst = p.o + (size_t)(q.row0 + tok) * p.ldo +
-                           (size_t)(head * p.group + rt % p.group) * D;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        *reinterpret_cast<uint32_t*>(dst + (e * 32 + lane) * 2) =
-            sees ? pack_bf16(acc[e].x * norm, acc[e].y * norm) : 0u;
-    }
+    if (r < rows && mine == 0) kv_put_row<D>(p, q, head, tile * TR + r, acc, l);
   }
 }
 
@@ -1330,15 +1406,40 @@ int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
   p.c = a.scale * 1.4426950408889634f;
   p.err = err;
   const int slots = slot_count(p.rows * p.group, p.seqs, 8 * NR, 1);
+  const long long tiles = (long long)slots * p.kv_heads;
+  const long long reach = a.window > 0 && a.window < a.max_len - p.rows ? (long long)a.window + p.rows
+                                                                       : a.max_len;
+  const long long units = (reach + C::kTok - 1) / C::kTok;          // of a tile, at most
+  // A block a tile (TEAM) where the tiles fit the SMs and the longest is short: 5 us and
+  // 1.3 to 1.8 for each stage of a warp, against 9 us and the bytes at HBM's rate for
+  // equal runs of all the work.  Measured, one token a sequence at head width 128, 4
+  // query heads a key head, us (TEAM / equal runs):
+  //   tokens        300          1000          2000         4000
+  //   8 tiles     6.2 /  8.2    9.6 /  9.2   15.6 /  9.4   24.1 / 10.0
+  //   32          6.6 / 11.8   10.1 / 12.3   16.2 / 14.4   24.9 / 16.8
+  //   64          6.7 / 11.0   10.4 / 15.3   16.8 / 19.4   25.6 / 24.4
+  // and not beyond 6 stages a warp, since lengths may be anything up to max_len.
+  const long long used = p.rows == p.seqs ? (long long)p.seqs * ((p.group + 8 * NR - 1) / (8 * NR))
+                                          : slots;                  // slots with rows
+  const long long rounds = (units + C::kWarps - 1) / C::kWarps;
+  if (used * p.kv_heads <= num_sms && p.seqs <= C::kThreads && rounds <= 6 &&
+      (rounds - 3) * 1200 <= NR * used * p.kv_heads * units) {
+    static std::atomic<unsigned long long> attr{0};
+    if (!smem_limit_once(kv8_attention_kernel<D, NR, true>, C::kSmem, attr)) return -1;
+    launch_k(kv8_attention_kernel<D, NR, true>, dim3((unsigned)tiles), dim3(C::kThreads), C::kSmem,
+             s, 1, p);
+    return launched();
+  }
   // a block for each SM, fewer where the longest sequences cannot fill them
-  const long long units = (long long)slots * p.kv_heads * ((a.max_len + C::kTok - 1) / C::kTok + 1);
-  const int grid = (int)(units < num_sms ? (units < 1 ? 1 : units) : num_sms);
+  const long long most = tiles * (units + 1);
+  const int grid = (int)(most < num_sms ? (most < 1 ? 1 : most) : num_sms);
   p.workers = grid * C::kWarps;
   p.part_o = a.workspace;
   p.part_ml = p.part_o + (size_t)p.workers * 2 * (8 * NR) * D;
   static std::atomic<unsigned long long> attr{0};
-  if (!smem_limit_once(kv8_attention_kernel<D, NR>, C::kSmem, attr)) return -1;
-  launch_k(kv8_attention_kernel<D, NR>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1, p);
+  if (!smem_limit_once(kv8_attention_kernel<D, NR, false>, C::kSmem, attr)) return -1;
+  launch_k(kv8_attention_kernel<D, NR, false>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1,
+           p);
   if (launched() != 0) return -1;
   // few tiles have many parts each: 16 warps a row (1 sequence of 131072 tokens, 222
   // parts a row: 53.5 us with the attention, 54.8 with 32 warps, 57.1 with 8); else a
