@@ -213,6 +213,73 @@ def test_more_items_than_sms(ctx, D, heads, kv_heads, causal, window, prefix, se
     check(got, want, tol, cu_q)
 
 
+LONG = [
+    # lens_q, lens_k
+    ([1], [4500]),
+    ([64], [8200]),
+    ([3, 40, 0, 130], [9000, 5000, 70, 12000]),
+    ([70, 10, 200], [10, 20000, 0]),          # rows that see nothing beside a long sequence
+    ([128, 1], [2049, 16384]),
+]
+
+
+@pytest.mark.parametrize("lens_q,lens_k", LONG)
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 8, 1), (64, 3, 3), (128, 8, 2), (128, 5, 1),
+                                              (256, 4, 2), (256, 1, 1)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 3001), (False, 0), (False, 7000)])
+def test_few_rows_over_long_keys(ctx, lens_q, lens_k, D, heads, kv_heads, causal, window):
+    """Keys that several SMs share, with NaN and infinities behind the last key."""
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 31, 3.0, pad=140)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=torch.bfloat16)
+    for x in (k, v):
+        x[cu_k[-1]:] = bad[torch.arange(140, device="cuda") % 3][:, None]
+    out = torch.full((q.shape[0], heads * D), 7.0, device="cuda", dtype=torch.bfloat16)
+    L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D, causal=causal,
+                       window=window, out=out)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, causal, window,
+                                        D ** -0.5)
+    check(out, want, tol, cu_q)
+    assert torch.all(out[cu_q[-1]:] == 7.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_rows_over_long_keys_captured(ctx, D):
+    """The same bits again, and a graph replayed with other lengths, some of them short;
+    NaN in values that only some rows see."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads = 4, 2
+    q, k, v, _, _ = make([80], [16000], heads, kv_heads, D, 5)
+    v[15990, 3] = math.nan
+    cq, ck = dev([0, 50, 80]), dev([0, 9000, 16000])
+    args = (ctx, q, k, v, cq, ck, heads, kv_heads, D)
+    a, b = L.attention_packed(*args), L.attention_packed(*args)
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        L.attention_packed(*args, out=out)
+    for lq, lk in (([0, 50, 80], [0, 9000, 16000]), ([0, 1, 80], [0, 15900, 16000]),
+                   ([5, 80, 80], [0, 100, 100]), ([0, 80, 80], [0, 0, 16000])):
+        cq.copy_(dev(lq))
+        ck.copy_(dev(lk))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        ctx.check()
+        want, tol = lm_ref.attention_packed(q, k, v, lq, lk, heads, kv_heads, D, True, 0, D ** -0.5)
+        rows = slice(lq[0], lq[-1])
+        assert torch.equal(out[rows].isnan(), want[rows].isnan())
+        ok = ~want[rows].isnan()
+        assert float(((out[rows].double() - want[rows]).abs() - tol[rows])[ok].max()) <= 1e-30
+        assert torch.all(out[:lq[0]] == 7.0) and torch.all(out[lq[-1]:] == 7.0)
+
+
 def test_rows_of_one_projection_and_other_streams(ctx):
     """q, k and v as column slices of one buffer, on a stream of the caller's."""
     import torch

@@ -118,6 +118,7 @@ struct PkParams {
   int kv_heads, group, tq;  // tq: tokens of a query tile
   int causal, window;
   int by_reach;             // items in the order of PkOrder
+  int split;                // CTAs that share an item's keys
   float c;                  // scale log2 e
   int* err;
 };
@@ -436,7 +437,99 @@ __device__ __forceinline__ int next_index(const void* answer)
   return ok != 0 ? (int)x : -1;
 }
 
-template <int D, bool NARROW>
+constexpr int kMaxSplit = 8;      // CTAs of a cluster
+
+__device__ __forceinline__ float2 ld_dsmem_f2(uint32_t caddr)
+{
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(caddr)
+               : "memory");
+  return v;
+}
+
+// Where 16-byte piece c of row `row` of a CTA's part of O lies.
+template <int D>
+__device__ __forceinline__ uint32_t pk_part(int row, int c)
+{
+  return (uint32_t)(row * (D / 4) + (c ^ (row & 7))) * 16u;
+}
+
+// This CTA's share of an item's rows out of the parts of all CTAs of the cluster: with
+// M the largest of their maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, in the
+// CTAs' order.  A thread has 4 columns at a time, a warp whole rows or 128 columns.
+template <int D, int T>
+__device__ __forceinline__ void pk_join(const PkParams& p, const PkItem& w, uint32_t parts,
+                                        uint32_t sums, int tid, int threads)
+{
+  constexpr int kPieces = D / 4, kSpan = D < 128 ? D : 128;
+  const int split = p.split, share = kRows / split, rank = (int)cluster_ctarank();
+  for (int u = tid; u < T * share * kPieces; u += threads) {
+    const int c = u % kPieces, t = u / kPieces / share, r = rank * share + u / kPieces % share;
+    const int place = t * kRows + r;
+    const int tok = w.tok0 + t * p.tq + r / p.group, shift = w.nk - w.nq;
+    const bool valid = r < p.tq * p.group && tok < w.nq;
+    const int lo = key_low(shift + tok, p.window);
+    const int hi = valid ? key_high(shift + tok, w.nk, p.causal) : 0;
+    float2 ml[kMaxSplit];
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMaxSplit; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.0f);
+      if (k < split)
+        ml[k] = ld_dsmem_f2(mapa_shared(sums + (uint32_t)place * 8u, (uint32_t)k));
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxSplit; ++k) top = fmaxf(top, ml[k].x);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k0 = 0; k0 < kMaxSplit; k0 += 4) {
+      float4 o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // a CTA that saw nothing of the row may have no O there
+        const bool none = ml[k0 + k].x == -INFINITY && ml[k0 + k].y == 0.0f;
+        o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!none) o[k] = ld_dsmem_f4(mapa_shared(parts + pk_part<D>(place, c), (uint32_t)(k0 + k)));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 y = ml[k0 + k];
+        const float f = y.x == -INFINITY ? 1.0f : fast_exp2(y.x - top);
+        l = fmaf(f, y.y, l);
+        acc.x = fmaf(f, o[k].x, acc.x);
+        acc.y = fmaf(f, o[k].y, acc.y);
+        acc.z = fmaf(f, o[k].z, acc.z);
+        acc.w = fmaf(f, o[k].w, acc.w);
+      }
+    }
+    const bool sees = hi > lo;
+    const float g = 1.0f / l;
+    const float x0 = sees ? acc.x * g : 0.0f, x1 = sees ? acc.y * g : 0.0f;
+    const float x2 = sees ? acc.z * g : 0.0f, x3 = sees ? acc.w * g : 0.0f;
+    const int row = w.row0 + tok, head = w.head * p.group + r % p.group;
+    if (valid)
+      *reinterpret_cast<uint2*>(p.o + (size_t)row * p.ldo + (size_t)head * D + c * 4) =
+          make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
+    const bool nan = x0 != x0 || x1 != x1 || x2 != x2 || x3 != x3;
+    __syncwarp();                                      // repair_row follows on these stores
+    // one lane of each row asks
+    uint32_t bad = __ballot_sync(0xffffffffu, nan && valid && l > 0.0f);
+    while (bad != 0) {
+      const int src = __ffs((int)bad) - 1;
+      bad &= kPieces < 32 ? ~(((1u << (kPieces & 31)) - 1u) << (src / kPieces * kPieces)) : 0u;
+      repair_row<D, kSpan>(p, __shfl_sync(0xffffffffu, row, src),
+                           __shfl_sync(0xffffffffu, head, src), w.head, w.key0,
+                           __shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src),
+                           __shfl_sync(0xffffffffu, c * 4 / kSpan * kSpan, src));
+    }
+  }
+}
+
+// SPLIT: a cluster of p.split CTAs has one item, each a run of its key tiles, and
+// ends with it.
+template <int D, bool NARROW, bool SPLIT>
 __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     pk_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k,
@@ -537,11 +630,11 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     const int slots = slot_count(p.rows, p.seqs, T * p.tq, 1);
     PkOrder order;
     if (p.by_reach) order.read(p, T * p.tq);
-    int index = (int)blockIdx.x;
+    int index = (int)(SPLIT ? blockIdx.x / (unsigned)p.split : blockIdx.x);
     bool ok = true;
     for (int it = 0; ok; ++it) {
       // the answer is read before the next question goes out to its place
-      if (index >= 0 && lane == 0) {
+      if (!SPLIT && index >= 0 && lane == 0) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         ask_next(s_answer, asked);
       }
@@ -582,6 +675,14 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
             w.tiles[t] = end > w.first ? (end - w.first + kKeys - 1) / kKeys : 0;
           }
         }
+        if constexpr (SPLIT) {
+          const int n = max(max(w.tiles[0], w.tiles[1]), max(w.tiles[2], w.tiles[3]));
+          const u64 rank = cluster_ctarank(), of = (u64)p.split;
+          const int from = (int)work_bound((u64)n, of, rank), to = (int)work_bound((u64)n, of, rank + 1);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) w.tiles[t] = clamp_int(w.tiles[t] - from, 0, to - from);
+          w.first += from * kKeys;
+        }
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u,
                                              s_abort, p.err, PERR_ITEM));
@@ -590,6 +691,10 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         mbar_arrive(&item_full[it & 1]);
       }
       if (index < 0) break;
+      if (SPLIT) {
+        index = -1;
+        continue;
+      }
       // every question is waited for, so that no answer is under way at the end
       volatile int no_abort = 0;
       const bool told = __all_sync(
@@ -831,7 +936,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     const float c = p.c;
     // score tiles of this query tile so far, and exchanges (kSplit 2)
     uint32_t step = 0, swap = 0, closed = 0;           // closed: items with keys
-    bool ok = true;
+    bool ok = true, joins = false;
 #pragma unroll 1
     for (int it = 0;; ++it) {
       // Two warps a row meet at barriers, so all warps of a tile agree on going on:
@@ -977,10 +1082,9 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         if (ok && lane == 0) mbar_arrive(&p_full[sb]);
       }
       // the row's sum over its threads, under the last maximum
-      float l_row = l_run;
+      float l_row = l_run, m_end = m_run;
       if (kAlt == 2 && nt > 0) {
         const uint32_t end = step + (uint32_t)nt - 1u;
-        float m_end = m_run;
         if ((int)(end & 1u) != alt) {
           ok = __all_sync(0xffffffffu,
                           ok && mbar_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
@@ -1013,6 +1117,30 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
                                                        PERR_SOFTMAX));
         ++closed;
       }
+      if constexpr (SPLIT) {
+        // O and (maximum, sum) to this CTA's shared memory, once the products of all
+        // query tiles are through with it; 16-byte pieces in turn against bank conflicts
+        constexpr int kCols = D / kSplit;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(drain, 0, s_abort, p.err, PERR_SOFTMAX));
+        if (ok && stores) {
+          tc_fence_after();
+#pragma unroll
+          for (int c4 = 0; c4 < kCols / 32; ++c4) {
+            uint32_t v[32];
+            tmem_ld32(orow + (uint32_t)(hh * kCols + c4 * 32), v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(
+                  s_ring + pk_part<D>(t * kRows + r, hh * (kCols / 4) + c4 * 8 + e)) =
+                  make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+          if (hh == 0)                                 // (Q's place)
+            reinterpret_cast<float2*>(s_q)[t * kRows + r] = make_float2(m_end, nt > 0 ? l_row : 0.0f);
+        }
+        joins = true;
+        break;
+      }
       if (!ok) continue;
       if (stores) {
         tc_fence_after();
@@ -1041,6 +1169,16 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[it & 1]);
     }
+    if constexpr (SPLIT) {
+      cluster_sync_all();                              // every CTA's part is there
+      if (joins)
+        pk_join<D, T>(p, s_item[0], smem_u32(s_ring), smem_u32(s_q), (int)threadIdx.x - 128,
+                      C::kThreads - 128);
+    }
+  }
+  if constexpr (SPLIT) {
+    if (warp < 4) cluster_sync_all();
+    cluster_sync_all();                                // parts are read, CTAs may go
   }
   tc_fence_before();
   __syncthreads();
@@ -1076,8 +1214,8 @@ bool pk_encode(CUtensorMap* map, const __nv_bfloat16* x, int D, int heads, int r
 
 constexpr long long kOrderBytes = 96ll << 20;    // keys and values that stay in L2 (126 MB)
 
-template <int D, bool NARROW>
-int pk_launch(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
+template <int D, bool NARROW, bool SPLIT>
+int pk_launch(const PackedAttention& a, int num_sms, int split, int* err, cudaStream_t s)
 {
   using C = PkCfg<D, NARROW>;
   PkParams p;
@@ -1111,14 +1249,50 @@ int pk_launch(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
     return -1;
   const long long grid =
       (long long)slot_count(a.rows, a.seqs, C::kTiles * p.tq, 1) * a.kv_heads;
-  if (grid > INT_MAX) return -2;
+  if (grid * split > INT_MAX) return -2;
   p.by_reach = a.seqs > 1 && a.seqs <= 32 && grid > num_sms &&
                (D == 64 || (long long)a.keys * a.kv_heads * (D * 4) <= kOrderBytes);
   static std::atomic<unsigned long long> attr{0};
-  if (!smem_limit_once(pk_attention_kernel<D, NARROW>, C::kSmem, attr)) return -1;
-  launch_k(pk_attention_kernel<D, NARROW>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, s, 1,
-           mq, mk, mv, p);
+  if (!smem_limit_once(pk_attention_kernel<D, NARROW, SPLIT>, C::kSmem, attr)) return -1;
+  p.split = split;
+  launch_k(pk_attention_kernel<D, NARROW, SPLIT>, dim3((unsigned)(grid * split)), dim3(C::kThreads),
+           C::kSmem, s, split, mq, mk, mv, p);
   return launched();
+}
+
+// CTAs an item: where the items alone leave SMs idle, or a last round of them nearly so,
+// and the keys are long, clusters share them.  A shared item costs its start and join
+// again.
+template <int D>
+int pk_split(const PackedAttention& a, long long items, int num_sms)
+{
+  constexpr int kKeys = PkCfg<D, D == 128>::kKeys;
+  constexpr float kStep = D == 128 ? 0.8f : 1.9f;      // us a key tile
+  constexpr float kStart = 6.0f;
+  float keys = (float)a.keys / (float)a.seqs;
+  if (a.window > 0) keys = fminf(keys, (float)a.window + (float)kRows);
+  const float tiles = keys / (float)kKeys;
+  float best = 0.9f * (float)((items + num_sms - 1) / num_sms) * tiles * kStep;
+  int split = 1;
+  for (int n = 2; n <= kMaxSplit; n *= 2) {
+    const float t = (float)((items * n + num_sms - 1) / num_sms) * (tiles / (float)n * kStep + kStart);
+    if (t < best) {
+      best = t;
+      split = n;
+    }
+  }
+  return split;
+}
+
+template <int D, bool NARROW>
+int pk_form(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
+{
+  const int tq = kRows / (a.heads / a.kv_heads);
+  const long long items =
+      (long long)slot_count(a.rows, a.seqs, PkCfg<D, NARROW>::kTiles * tq, 1) * a.kv_heads;
+  const int split = pk_split<D>(a, items, num_sms);
+  return split > 1 ? pk_launch<D, NARROW, true>(a, num_sms, split, err, s)
+                   : pk_launch<D, NARROW, false>(a, num_sms, 1, err, s);
 }
 
 }  // namespace
@@ -1126,14 +1300,14 @@ int pk_launch(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
 int launch_attention_packed(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
 {
   switch (a.head_dim) {
-    case 64: return pk_launch<64, false>(a, num_sms, err, s);
+    case 64: return pk_form<64, false>(a, num_sms, err, s);
     case 128: {
       const int tq = kRows / (a.heads / a.kv_heads);
       const long long wide = (long long)slot_count(a.rows, a.seqs, 2 * tq, 1) * a.kv_heads;
-      return wide <= num_sms ? pk_launch<128, true>(a, num_sms, err, s)
-                             : pk_launch<128, false>(a, num_sms, err, s);
+      return wide <= num_sms ? pk_form<128, true>(a, num_sms, err, s)
+                             : pk_launch<128, false, false>(a, num_sms, 1, err, s);
     }
-    case 256: return pk_launch<256, false>(a, num_sms, err, s);
+    case 256: return pk_form<256, false>(a, num_sms, err, s);
     default: return -2;
   }
 }
