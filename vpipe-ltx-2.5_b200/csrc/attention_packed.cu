@@ -28,6 +28,9 @@
 // loads and first scores run under this one's last softmax and store, and the
 // items, longest first in a causal sequence or in the whole call (PkOrder), go to
 // whoever is free.
+// Few items over long keys (a prompt's next chunk) go to clusters of 2, 4 or 8 CTAs,
+// each with a run of the keys; their parts of O are joined through distributed shared
+// memory (pk_join), so that no workspace is needed.
 // With several tiles one's MMAs run under the others' softmax; with one tile the
 // scores are double-buffered, so S of key tile j + 1 runs under softmax j.
 // V is used as TMA lays it down, [key][64 dims] in 128-byte swizzled rows: the
@@ -456,73 +459,97 @@ __device__ __forceinline__ uint32_t pk_part(int row, int c)
   return (uint32_t)(row * (D / 4) + (c ^ (row & 7))) * 16u;
 }
 
-// This CTA's share of an item's rows out of the parts of all CTAs of the cluster: with
-// M the largest of their maxima, o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, in the
-// CTAs' order.  A thread has 4 columns at a time, a warp whole rows or 128 columns.
-template <int D, int T>
+// This CTA's share of an item's rows (every S-th) out of the parts of the S CTAs of
+// the cluster: with M the largest of their maxima,
+//   o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i,
+// in the CTAs' order.  A thread has 4 columns at a time, a warp whole rows or 128
+// columns, and asks for 4 parts at once.
+template <int D, int T, int S>
 __device__ __forceinline__ void pk_join(const PkParams& p, const PkItem& w, uint32_t parts,
                                         uint32_t sums, int tid, int threads)
 {
   constexpr int kPieces = D / 4, kSpan = D < 128 ? D : 128;
-  const int split = p.split, share = kRows / split, rank = (int)cluster_ctarank();
-  for (int u = tid; u < T * share * kPieces; u += threads) {
-    const int c = u % kPieces, t = u / kPieces / share, r = rank * share + u / kPieces % share;
-    const int place = t * kRows + r;
-    const int tok = w.tok0 + t * p.tq + r / p.group, shift = w.nk - w.nq;
-    const bool valid = r < p.tq * p.group && tok < w.nq;
-    const int lo = key_low(shift + tok, p.window);
-    const int hi = valid ? key_high(shift + tok, w.nk, p.causal) : 0;
-    float2 ml[kMaxSplit];
-    float top = -INFINITY, l = 0.0f;
+  constexpr int kBatch = S < 4 ? S : 4, kAhead = 4 / kBatch;
+  constexpr int kShare = kRows / S, kTotal = T * kShare * kPieces;
+  const int rank = (int)cluster_ctarank(), rows = p.tq * p.group, shift = w.nk - w.nq;
+#pragma unroll 1
+  for (int u0 = tid; u0 < kTotal; u0 += kAhead * threads) {
+    float2 ml[kAhead][S];
+    float4 o[kAhead][kBatch];
+    uint32_t part[kAhead];
+    int at[kAhead];                                    // the row's place in its item, or -1
+    bool any = false;
 #pragma unroll
-    for (int k = 0; k < kMaxSplit; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.0f);
-      if (k < split)
-        ml[k] = ld_dsmem_f2(mapa_shared(sums + (uint32_t)place * 8u, (uint32_t)k));
-    }
-#pragma unroll
-    for (int k = 0; k < kMaxSplit; ++k) top = fmaxf(top, ml[k].x);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int k0 = 0; k0 < kMaxSplit; k0 += 4) {
-      float4 o[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // a CTA that saw nothing of the row may have no O there
-        const bool none = ml[k0 + k].x == -INFINITY && ml[k0 + k].y == 0.0f;
-        o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (!none) o[k] = ld_dsmem_f4(mapa_shared(parts + pk_part<D>(place, c), (uint32_t)(k0 + k)));
+    for (int i = 0; i < kAhead; ++i) {
+      const int u = u0 + i * threads, n = u / kPieces;
+      const int t = n / kShare, r = n % kShare * S + rank;
+      at[i] = -1;
+      if (u < kTotal && r < rows) {
+        const int tok = t * p.tq + r / p.group;
+        if (w.tok0 + tok < w.nq) at[i] = tok * p.group + r % p.group;
       }
+      if (at[i] >= 0) {
+        any = true;
+        const int place = t * kRows + r;
+        const uint32_t sum = sums + (uint32_t)place * 8u;
+        part[i] = parts + pk_part<D>(place, u % kPieces);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 y = ml[k0 + k];
-        const float f = y.x == -INFINITY ? 1.0f : fast_exp2(y.x - top);
-        l = fmaf(f, y.y, l);
-        acc.x = fmaf(f, o[k].x, acc.x);
-        acc.y = fmaf(f, o[k].y, acc.y);
-        acc.z = fmaf(f, o[k].z, acc.z);
-        acc.w = fmaf(f, o[k].w, acc.w);
+        for (int k = 0; k < S; ++k) ml[i][k] = ld_dsmem_f2(mapa_shared(sum, (uint32_t)k));
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) o[i][k] = ld_dsmem_f4(mapa_shared(part[i], (uint32_t)k));
       }
     }
-    const bool sees = hi > lo;
-    const float g = 1.0f / l;
-    const float x0 = sees ? acc.x * g : 0.0f, x1 = sees ? acc.y * g : 0.0f;
-    const float x2 = sees ? acc.z * g : 0.0f, x3 = sees ? acc.w * g : 0.0f;
-    const int row = w.row0 + tok, head = w.head * p.group + r % p.group;
-    if (valid)
-      *reinterpret_cast<uint2*>(p.o + (size_t)row * p.ldo + (size_t)head * D + c * 4) =
-          make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
-    const bool nan = x0 != x0 || x1 != x1 || x2 != x2 || x3 != x3;
-    __syncwarp();                                      // repair_row follows on these stores
-    // one lane of each row asks
-    uint32_t bad = __ballot_sync(0xffffffffu, nan && valid && l > 0.0f);
-    while (bad != 0) {
-      const int src = __ffs((int)bad) - 1;
-      bad &= kPieces < 32 ? ~(((1u << (kPieces & 31)) - 1u) << (src / kPieces * kPieces)) : 0u;
-      repair_row<D, kSpan>(p, __shfl_sync(0xffffffffu, row, src),
-                           __shfl_sync(0xffffffffu, head, src), w.head, w.key0,
-                           __shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src),
-                           __shfl_sync(0xffffffffu, c * 4 / kSpan * kSpan, src));
+    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int c = (u0 + i * threads) % kPieces;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float l = 0.0f;
+      int lo = 0, hi = 0, row = 0, head = 0;
+      if (at[i] >= 0) {
+        const int tok = w.tok0 + at[i] / p.group;
+        row = w.row0 + tok;
+        head = w.head * p.group + at[i] % p.group;
+        lo = key_low(shift + tok, p.window);
+        hi = key_high(shift + tok, w.nk, p.causal);
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < S; ++k) top = fmaxf(top, ml[i][k].x);
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+          if (k > 0 && k % kBatch == 0) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+              o[i][j] = ld_dsmem_f4(mapa_shared(part[i], (uint32_t)(k + j)));
+          }
+          const float2 y = ml[i][k];
+          const float4 z = o[i][k % kBatch];
+          if (y.x == -INFINITY && y.y == 0.0f) continue; // saw nothing; what was read is no O
+          const float f = y.x == -INFINITY ? 1.0f : fast_exp2(y.x - top);
+          l = fmaf(f, y.y, l);
+          x.x = fmaf(f, z.x, x.x);
+          x.y = fmaf(f, z.y, x.y);
+          x.z = fmaf(f, z.z, x.z);
+          x.w = fmaf(f, z.w, x.w);
+        }
+        const float g = 1.0f / l;
+        x = hi > lo ? make_float4(x.x * g, x.y * g, x.z * g, x.w * g)
+                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<uint2*>(p.o + (size_t)row * p.ldo + (size_t)head * D + c * 4) =
+            make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+      }
+      const bool nan = x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
+      __syncwarp();                                    // repair_row follows on these stores
+      // one lane of each row asks
+      uint32_t bad = __ballot_sync(0xffffffffu, nan && l > 0.0f);
+      while (bad != 0) {
+        const int src = __ffs((int)bad) - 1;
+        bad &= kPieces < 32 ? ~(((1u << (kPieces & 31)) - 1u) << (src / kPieces * kPieces)) : 0u;
+        repair_row<D, kSpan>(p, __shfl_sync(0xffffffffu, row, src),
+                             __shfl_sync(0xffffffffu, head, src), w.head, w.key0,
+                             __shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src),
+                             __shfl_sync(0xffffffffu, c * 4 / kSpan * kSpan, src));
+      }
     }
   }
 }
@@ -1171,9 +1198,13 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     }
     if constexpr (SPLIT) {
       cluster_sync_all();                              // every CTA's part is there
-      if (joins)
-        pk_join<D, T>(p, s_item[0], smem_u32(s_ring), smem_u32(s_q), (int)threadIdx.x - 128,
-                      C::kThreads - 128);
+      if (joins) {
+        const uint32_t parts = smem_u32(s_ring), sums = smem_u32(s_q);
+        const int tid = (int)threadIdx.x - 128, threads = C::kThreads - 128;
+        if (p.split == 2) pk_join<D, T, 2>(p, s_item[0], parts, sums, tid, threads);
+        else if (p.split == 4) pk_join<D, T, 4>(p, s_item[0], parts, sums, tid, threads);
+        else pk_join<D, T, 8>(p, s_item[0], parts, sums, tid, threads);
+      }
     }
   }
   if constexpr (SPLIT) {
@@ -1260,22 +1291,62 @@ int pk_launch(const PackedAttention& a, int num_sms, int split, int* err, cudaSt
   return launched();
 }
 
-// CTAs an item: where the items alone leave SMs idle, or a last round of them nearly so,
-// and the keys are long, clusters share them.  A shared item costs its start and join
-// again.
-template <int D>
+// Clusters of n CTAs that the current device holds at once (0: none), asked once.
+template <int D, bool NARROW>
+int pk_clusters(int n)
+{
+  using C = PkCfg<D, NARROW>;
+  static std::atomic<int> known[64][kMaxSplit + 1];    // count + 1
+  static std::atomic<unsigned long long> attr{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int have = known[dev][n].load(std::memory_order_relaxed);
+  if (have == 0) {
+    if (!smem_limit_once(pk_attention_kernel<D, NARROW, true>, C::kSmem, attr)) return 0;
+    cudaLaunchAttribute size;
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = (unsigned)n;
+    size.val.clusterDim.y = size.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.attrs = &size;
+    cfg.numAttrs = 1;
+    int count = 0;
+    if (cudaOccupancyMaxActiveClusters(&count, pk_attention_kernel<D, NARROW, true>, &cfg) !=
+        cudaSuccess) {
+      cudaGetLastError();
+      count = 0;
+    }
+    have = count + 1;
+    known[dev][n].store(have, std::memory_order_relaxed);
+  }
+  return have - 1;
+}
+
+// CTAs an item: where the items alone leave SMs idle and the keys are long, clusters
+// share them.  Measured: a key tile takes kStep us, the join kJoin, and a further
+// round of clusters, which start anew, 12 (a CTA on its own goes on to its next item).
+// 32/8 heads of 128, one sequence, us (alone / by the rule):
+//   new tokens, keys before      500           2000          8000          32000
+//   16                        9.6 /  8.6   19.1 /  9.8   56.1 / 15.9   204.3 / 35.6
+//   64                       11.1 / 10.7   19.8 / 12.4   58.0 / 23.1   206.7 / 61.8
+template <int D, bool NARROW>
 int pk_split(const PackedAttention& a, long long items, int num_sms)
 {
-  constexpr int kKeys = PkCfg<D, D == 128>::kKeys;
-  constexpr float kStep = D == 128 ? 0.8f : 1.9f;      // us a key tile
-  constexpr float kStart = 6.0f;
+  constexpr float kStep = D == 128 ? 0.82f : 1.33f;
+  constexpr float kJoin = D == 64 ? 4.3f : D == 128 ? 2.5f : 6.3f, kRound = 12.0f;
   float keys = (float)a.keys / (float)a.seqs;
   if (a.window > 0) keys = fminf(keys, (float)a.window + (float)kRows);
-  const float tiles = keys / (float)kKeys;
-  float best = 0.9f * (float)((items + num_sms - 1) / num_sms) * tiles * kStep;
+  const float alone = keys / (float)PkCfg<D, NARROW>::kKeys * kStep;      // us an item
+  float best = 0.95f * (float)((items + num_sms - 1) / num_sms) * alone;
   int split = 1;
-  for (int n = 2; n <= kMaxSplit; n *= 2) {
-    const float t = (float)((items * n + num_sms - 1) / num_sms) * (tiles / (float)n * kStep + kStart);
+  for (int n = 2; n <= kMaxSplit && kJoin + alone / (float)n < best; n *= 2) {
+    const int fit = pk_clusters<D, NARROW>(n);
+    if (fit <= 0) break;
+    const float rounds = (float)((items + fit - 1) / fit);
+    const float t = kJoin + rounds * alone / (float)n + (rounds - 1.0f) * kRound;
     if (t < best) {
       best = t;
       split = n;
@@ -1290,7 +1361,7 @@ int pk_form(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
   const int tq = kRows / (a.heads / a.kv_heads);
   const long long items =
       (long long)slot_count(a.rows, a.seqs, PkCfg<D, NARROW>::kTiles * tq, 1) * a.kv_heads;
-  const int split = pk_split<D>(a, items, num_sms);
+  const int split = pk_split<D, NARROW>(a, items, num_sms);
   return split > 1 ? pk_launch<D, NARROW, true>(a, num_sms, split, err, s)
                    : pk_launch<D, NARROW, false>(a, num_sms, 1, err, s);
 }
