@@ -355,7 +355,9 @@ LTX_API int ltx_attention(ltx_ctx* ctx, const void* q, int ldq, const void* k,
  *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j),
  * zero where it sees none.  What lies outside a row's keys does not reach it,
  * whatever it holds (NaN and infinities too).  Rows outside the sequences are
- * left as they are.  o must not overlap q, k or v.  Allocates nothing. */
+ * left as they are.  o must not overlap q, k or v.  The launch is sized for
+ * keys / seqs keys a sequence; any lengths within `keys` are right.  Allocates
+ * nothing. */
 LTX_API int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const void* k, int ldk,
                                  const void* v, int ldv, void* o, int ldo, const int32_t* cu_q,
                                  const int32_t* cu_k, int seqs, int rows, int keys, int heads,
@@ -412,8 +414,10 @@ LTX_API int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int 
  * result is ltx_attention_packed's over the values the codes stand for (an
  * infinity in a row of q makes that row NaN).  o must not overlap q.  One
  * token a sequence is the usual call; the cache is read once for each 16 rows
- * (tokens times the query heads of a key/value head).  max_len sizes the
- * launch: the largest length expected.  The workspace is the caller's,
+ * (tokens times the query heads of a key/value head), at head_dim 256 for each
+ * 8, so that many new tokens go better through ltx_kv8_read and
+ * ltx_attention_packed.  max_len sizes the launch: the largest length
+ * expected; longer ones are right too.  The workspace is the caller's,
  * ltx_kv8_attention_workspace bytes whatever the lengths, 16-byte aligned, of
  * any content; two calls that may run at once (streams, captured graphs) need
  * one each.  Allocates nothing. */

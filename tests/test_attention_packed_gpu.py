@@ -246,6 +246,19 @@ def test_few_rows_over_long_keys(ctx, lens_q, lens_k, D, heads, kv_heads, causal
     assert torch.all(out[cu_q[-1]:] == 7.0)
 
 
+def test_long_keys_shared_in_several_rounds(ctx):
+    """More items than SMs, each shared all the same, in the order of their keys."""
+    import torch
+    import ltx25_b200 as L
+    heads, kv_heads, D, lens_q, lens_k = 16, 8, 256, [600, 500], [13000, 12000]
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 33)
+    got = L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, True, 0, D ** -0.5)
+    check(got, want, tol, cu_q)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_few_rows_over_long_keys_captured(ctx, D):
     """The same bits again, and a graph replayed with other lengths, some of them short;
@@ -278,6 +291,49 @@ def test_few_rows_over_long_keys_captured(ctx, D):
         ok = ~want[rows].isnan()
         assert float(((out[rows].double() - want[rows]).abs() - tol[rows])[ok].max()) <= 1e-30
         assert torch.all(out[:lq[0]] == 7.0) and torch.all(out[lq[-1]:] == 7.0)
+
+
+FIRST = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import ltx25_b200 as L
+ctx = L.Context(0)
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+for D in (64, 128, 256):
+    q = torch.randn((40, 4 * D), device="cuda").to(torch.bfloat16)
+    k = torch.randn((9000, 2 * D), device="cuda").to(torch.bfloat16)
+    cu_q, cu_k, out = ints([0, 40]), ints([0, 9000]), torch.zeros_like(q)
+    cache = L.KV8Cache.empty(ctx, 4, 2, D)
+    cu, n, nine, t = ints([0, 9]), ints([0]), ints([9]), ints([[2, 0]])
+    back = torch.zeros((9, 4 * D), device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(L.kv8_attention_workspace(ctx, D), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        L.attention_packed(ctx, q, k, k, cu_q, cu_k, 4, 2, D, out=out)
+        L.kv8_append(ctx, cache, k[:9], k[:9], cu, n, t)
+        L.kv8_attention(ctx, cache, q[:9], cu, nine, t, 4, 128, out=back, workspace=ws)
+    g.replay()
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.equal(out, L.attention_packed(ctx, q, k, k, cu_q, cu_k, 4, 2, D))
+    assert torch.equal(back, L.kv8_attention(ctx, cache, q[:9], cu, nine, t, 4, 128))
+    for x in (out, back):
+        assert bool(x.isfinite().all()) and bool((x != 0).any())
+print("fine")
+"""
+
+
+def test_a_process_s_first_calls_may_be_captured(ctx):
+    """Whatever a kernel is asked once happens during a capture then."""
+    import os
+    import subprocess
+    import sys
+    import ltx25_b200
+    lib = os.path.dirname(os.path.dirname(os.path.abspath(ltx25_b200.__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST, lib], capture_output=True, text=True,
+                       timeout=600)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
 
 
 def test_rows_of_one_projection_and_other_streams(ctx):

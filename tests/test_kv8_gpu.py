@@ -260,6 +260,21 @@ def test_attention_of_short_sequences(ctx, D, heads, kv_heads, window):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("max_len", [0, 1, 300])
+def test_longer_than_expected(ctx, D, max_len):
+    """max_len sizes the launch; what a sequence holds beyond it counts all the same."""
+    import torch
+    import ltx25_b200 as L
+    new, lengths, heads, kv_heads = [1, 2, 1], [5000, 700, 3], 4, 2
+    cache, q, cu, table = attention_case(ctx, new, lengths, heads, kv_heads, D, 0)
+    got = L.kv8_attention(ctx, cache, q, ints(cu), ints(lengths), ints(table), heads, max_len)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = expect(cache, q, cu, lengths, table, heads, 0)
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("a,b", [(116, 100), (-90, -100), (100, 0)])
 def test_attention_under_powers_of_two(ctx, D, a, b):
     """q by 2^a against K's scales by 2^-a, V's scales by 2^b: the products are the

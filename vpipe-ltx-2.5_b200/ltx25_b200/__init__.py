@@ -944,7 +944,7 @@ def kv8_read(ctx, cache, cu, starts, table, rows, k=None, v=None, stream=None):
     else:
         ldk = _rows(ctx, k, cols, "k", rows)
     if v is None:
-        v, ldv = _new(ctx, stream, cache.v_scale, (rows, cols)), cols
+        v, ldv = _new(ctx, stream, k), cols
     else:
         ldv = _rows(ctx, v, cols, "v", rows)
     pt, tld = _table(ctx, table, seqs)
