@@ -259,6 +259,31 @@ def test_long_keys_shared_in_several_rounds(ctx):
     check(got, want, tol, cu_q)
 
 
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv_heads,D", [
+    ([777, 333], [7700, 7300], 20, 4, 128),
+    ([1000], [9000], 20, 4, 128),
+    ([5] * 8, [3000] * 8, 20, 20, 64),
+    ([5, 1, 3, 0, 9, 5, 5, 5], [3000, 3001, 6000, 100, 2, 7000, 3000, 0], 20, 20, 64),
+    ([5] * 8, [3000] * 8, 20, 20, 256),
+    ([3, 2] * 17, [2500, 1900] * 17, 5, 5, 256),
+])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 2100)])
+def test_a_last_round_of_few_items(ctx, lens_q, lens_k, heads, kv_heads, D, causal, window):
+    """Items that fill the SMs once and a little: the last ones are shared."""
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 35, pad=30)
+    out = torch.full((q.shape[0], heads * D), 7.0, device="cuda", dtype=torch.bfloat16)
+    args = (ctx, q, k, v, dev(cu_q), dev(cu_k), heads, kv_heads, D)
+    L.attention_packed(*args, causal=causal, window=window, out=out)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, D, causal, window,
+                                        D ** -0.5)
+    check(out, want, tol, cu_q)
+    assert torch.all(out[cu_q[-1]:] == 7.0)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_few_rows_over_long_keys_captured(ctx, D):
     """The same bits again, and a graph replayed with other lengths, some of them short;

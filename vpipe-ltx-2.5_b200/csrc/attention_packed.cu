@@ -121,6 +121,7 @@ struct PkParams {
   int kv_heads, group, tq;  // tq: tokens of a query tile
   int causal, window;
   int by_reach;             // items in the order of PkOrder
+  int base;                 // the grid's first item
   int split;                // CTAs that share an item's keys
   float c;                  // scale log2 e
   int* err;
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     const int slots = slot_count(p.rows, p.seqs, T * p.tq, 1);
     PkOrder order;
     if (p.by_reach) order.read(p, T * p.tq);
-    int index = (int)(SPLIT ? blockIdx.x / (unsigned)p.split : blockIdx.x);
+    int index = p.base + (int)(SPLIT ? blockIdx.x / (unsigned)p.split : blockIdx.x);
     bool ok = true;
     for (int it = 0; ok; ++it) {
       // the answer is read before the next question goes out to its place
@@ -727,7 +728,10 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       const bool told = __all_sync(
           0xffffffffu, mbar_wait(asked, (uint32_t)it & 1u, &no_abort, p.err, PERR_DRAIN));
       ok = ok && told;
-      if (ok) index = next_index(s_answer);
+      if (ok) {
+        index = next_index(s_answer);
+        if (index >= 0) index += p.base;
+      }
       __syncwarp();
     }
   } else if (warp == 0) {
@@ -1245,8 +1249,18 @@ bool pk_encode(CUtensorMap* map, const __nv_bfloat16* x, int D, int heads, int r
 
 constexpr long long kOrderBytes = 96ll << 20;    // keys and values that stay in L2 (126 MB)
 
+// The items of a call, and `count` of them from `base` on as one grid.
+template <int D, bool NARROW>
+long long pk_items(const PackedAttention& a)
+{
+  return (long long)slot_count(a.rows, a.seqs,
+                               PkCfg<D, NARROW>::kTiles * (kRows / (a.heads / a.kv_heads)), 1) *
+         a.kv_heads;
+}
+
 template <int D, bool NARROW, bool SPLIT>
-int pk_launch(const PackedAttention& a, int num_sms, int split, int* err, cudaStream_t s)
+int pk_launch(const PackedAttention& a, int num_sms, long long base, long long count, int split,
+              int* err, cudaStream_t s)
 {
   using C = PkCfg<D, NARROW>;
   PkParams p;
@@ -1278,15 +1292,14 @@ int pk_launch(const PackedAttention& a, int num_sms, int split, int* err, cudaSt
       !pk_encode(&mk, none ? a.q : a.k, D, a.kv_heads, none ? 1 : a.keys, a.ldk, 1, C::kKeys) ||
       !pk_encode(&mv, none ? a.q : a.v, D, a.kv_heads, none ? 1 : a.keys, a.ldv, 1, C::kVKeys))
     return -1;
-  const long long grid =
-      (long long)slot_count(a.rows, a.seqs, C::kTiles * p.tq, 1) * a.kv_heads;
-  if (grid * split > INT_MAX) return -2;
-  p.by_reach = a.seqs > 1 && a.seqs <= 32 && grid > num_sms &&
+  if (base + count > INT_MAX || count * split > INT_MAX) return -2;
+  p.by_reach = a.seqs > 1 && a.seqs <= 32 && pk_items<D, NARROW>(a) > num_sms &&
                (D == 64 || (long long)a.keys * a.kv_heads * (D * 4) <= kOrderBytes);
   static std::atomic<unsigned long long> attr{0};
   if (!smem_limit_once(pk_attention_kernel<D, NARROW, SPLIT>, C::kSmem, attr)) return -1;
+  p.base = (int)base;
   p.split = split;
-  launch_k(pk_attention_kernel<D, NARROW, SPLIT>, dim3((unsigned)(grid * split)), dim3(C::kThreads),
+  launch_k(pk_attention_kernel<D, NARROW, SPLIT>, dim3((unsigned)(count * split)), dim3(C::kThreads),
            C::kSmem, s, split, mq, mk, mv, p);
   return launched();
 }
@@ -1333,20 +1346,16 @@ int pk_clusters(int n)
 //   16                        9.6 /  8.6   19.1 /  9.8   56.1 / 15.9   204.3 / 35.6
 //   64                       11.1 / 10.7   19.8 / 12.4   58.0 / 23.1   206.7 / 61.8
 template <int D, bool NARROW>
-int pk_split(const PackedAttention& a, long long items, int num_sms)
+int pk_split(long long items, float alone, float start, int num_sms)
 {
-  constexpr float kStep = D == 128 ? 0.82f : 1.33f;
   constexpr float kJoin = D == 64 ? 4.3f : D == 128 ? 2.5f : 6.3f, kRound = 12.0f;
-  float keys = (float)a.keys / (float)a.seqs;
-  if (a.window > 0) keys = fminf(keys, (float)a.window + (float)kRows);
-  const float alone = keys / (float)PkCfg<D, NARROW>::kKeys * kStep;      // us an item
   float best = 0.95f * (float)((items + num_sms - 1) / num_sms) * alone;
   int split = 1;
-  for (int n = 2; n <= kMaxSplit && kJoin + alone / (float)n < best; n *= 2) {
+  for (int n = 2; n <= kMaxSplit && start + kJoin + alone / (float)n < best; n *= 2) {
     const int fit = pk_clusters<D, NARROW>(n);
     if (fit <= 0) break;
     const float rounds = (float)((items + fit - 1) / fit);
-    const float t = kJoin + rounds * alone / (float)n + (rounds - 1.0f) * kRound;
+    const float t = start + kJoin + rounds * alone / (float)n + (rounds - 1.0f) * kRound;
     if (t < best) {
       best = t;
       split = n;
@@ -1358,12 +1367,27 @@ int pk_split(const PackedAttention& a, long long items, int num_sms)
 template <int D, bool NARROW>
 int pk_form(const PackedAttention& a, int num_sms, int* err, cudaStream_t s)
 {
-  const int tq = kRows / (a.heads / a.kv_heads);
-  const long long items =
-      (long long)slot_count(a.rows, a.seqs, PkCfg<D, NARROW>::kTiles * tq, 1) * a.kv_heads;
-  const int split = pk_split<D, NARROW>(a, items, num_sms);
-  return split > 1 ? pk_launch<D, NARROW, true>(a, num_sms, split, err, s)
-                   : pk_launch<D, NARROW, false>(a, num_sms, 1, err, s);
+  constexpr float kStep = D == 128 ? 0.82f : 1.33f;
+  constexpr float kStart = 8.0f;                       // us of a second launch
+  float keys = (float)a.keys / (float)a.seqs;
+  if (a.window > 0) keys = fminf(keys, (float)a.window + (float)kRows);
+  const float alone = keys / (float)PkCfg<D, NARROW>::kKeys * kStep;      // us an item
+  const long long items = pk_items<D, NARROW>(a);
+  int split = pk_split<D, NARROW>(items, alone, 0.0f, num_sms);
+  if (split > 1) return pk_launch<D, NARROW, true>(a, num_sms, 0, items, split, err, s);
+  // items of about the same length that end in a round of few: these by clusters, in a
+  // launch of their own (2 chunks of 333 to 777 tokens on 6990, 20/4 heads of 128: 92
+  // against 101 us; 1200 tokens on 8000, 16/4 heads: 86 against 122)
+  const long long last = items % num_sms;
+  if (items > num_sms && last > 0 && (long long)a.rows * 2 <= a.keys) {
+    split = pk_split<D, NARROW>(last, alone, kStart, num_sms);
+    if (split > 1) {
+      const int rc = pk_launch<D, NARROW, false>(a, num_sms, 0, items - last, 1, err, s);
+      return rc != 0 ? rc
+                     : pk_launch<D, NARROW, true>(a, num_sms, items - last, last, split, err, s);
+    }
+  }
+  return pk_launch<D, NARROW, false>(a, num_sms, 0, items, 1, err, s);
 }
 
 }  // namespace
@@ -1373,10 +1397,9 @@ int launch_attention_packed(const PackedAttention& a, int num_sms, int* err, cud
   switch (a.head_dim) {
     case 64: return pk_form<64, false>(a, num_sms, err, s);
     case 128: {
-      const int tq = kRows / (a.heads / a.kv_heads);
-      const long long wide = (long long)slot_count(a.rows, a.seqs, 2 * tq, 1) * a.kv_heads;
+      const long long wide = pk_items<128, false>(a);
       return wide <= num_sms ? pk_form<128, true>(a, num_sms, err, s)
-                             : pk_launch<128, false, false>(a, num_sms, 1, err, s);
+                             : pk_launch<128, false, false>(a, num_sms, 0, wide, 1, err, s);
     }
     case 256: return pk_form<256, false>(a, num_sms, err, s);
     default: return -2;
