@@ -411,8 +411,10 @@ LTX_API int ltx_kv8_read(ltx_ctx* ctx, const ltx_kv8_cache* cache, void* k, int 
  * are the last tokens of sequence s, whose lengths[s] tokens (those included)
  * the cache holds; row i of n sees the tokens up to its own position
  * lengths[s] - n + i, with window > 0 only those above position - window.  The
- * result is ltx_attention_packed's over the values the codes stand for (an
- * infinity in a row of q makes that row NaN).  o must not overlap q.  One
+ * result is ltx_attention_packed's over the values the codes stand for, except
+ * that an infinity in a row of q makes that row NaN, and that values under
+ * 2^-64 times the largest v_scale among the pages that a sequence's rows see
+ * may count as zero.  o must not overlap q.  One
  * token a sequence is the usual call; the cache is read once for each 16 rows
  * (tokens times the query heads of a key/value head), at head_dim 256 for each
  * 8, so that many new tokens go better through ltx_kv8_read and

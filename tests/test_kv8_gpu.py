@@ -295,6 +295,57 @@ def test_attention_under_powers_of_two(ctx, D, a, b):
     assert bool(((got * 2.0 ** -b - near).abs() <= near.abs() * 2.0 ** -7).all())
 
 
+def steep_scales(exps, pages, kv_heads, table, lengths, seed):
+    """V scales of powers of two, those of a sequence's pages taking `exps` in turn (or
+    any of -133..60): bf16 [pages][kv_heads]."""
+    import torch
+    rng = np.random.default_rng(seed)
+    e = np.zeros((pages, kv_heads), dtype=np.int64)
+    for row, n in zip(table, lengths):
+        for b in range((n + 63) // 64):
+            for h in range(kv_heads):
+                e[row[b], h] = rng.integers(-133, 61) if exps is None else exps[(b + h) % len(exps)]
+    return torch.from_numpy(np.ldexp(1.0, e)).to(torch.bfloat16).cuda()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("exps", [(0, -120), (-5, -5, -110), (0, -133), (-133,), (-121, -128, -133),
+                                  (100, -20, -120, 40), (0, -60, 0, -70), None])
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,max_len", [
+    ([1, 2], [700, 1300], 8, 2, 1300), ([1, 3], [1900, 1300], 2, 2, 100000),
+    ([1] * 16, [2500] * 16, 8, 8, 2500), ([3] * 6, [150] * 6, 12, 2, 20000)])
+def test_attention_over_value_scales_at_the_ends_of_the_range(ctx, D, exps, new, lengths, heads,
+                                                              kv_heads, max_len):
+    """Pages whose V scales are up to 2^193 apart, subnormal ones among them.  Beside
+    lm_ref's bound, in units of a sequence's largest V scale T:
+      the lowest unit of O is max(2^-64 T / 32, 2^-126) or less; values of scales under
+      2^-8 of it count as zero, codes of 127 at most: 2^-70 T;
+      weights over the lowest unit round to 2^-25 of it a code: m 2^-18 of it for m
+      keys, over a sum of at least 1;
+      that lowest unit over the sum of weights (up to 2^6 m) may be subnormal: 2^-150 in
+      2^-126 / (2^6 m), m 2^-18 of the result;
+      and a bf16 result under 2^-126 rounds to 2^-134."""
+    import torch
+    import ltx25_b200 as L
+    cache, q, cu, table = attention_case(ctx, new, lengths, heads, kv_heads, D, 0)
+    scales = steep_scales(exps, cache.pages, kv_heads, table, lengths, 3)
+    cache = L.KV8Cache(cache.k, cache.v, cache.k_scale, scales)
+    got = L.kv8_attention(ctx, cache, q, ints(cu), ints(lengths), ints(table), heads, max_len)
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.isfinite(got).all()
+    k, v = values(cache.k, cache.k_scale), values(cache.v, scales)
+    for s, n in enumerate(lengths):
+        top = float(scales[table[s][:(n + 63) // 64]].double().max())
+        rows = slice(cu[s], cu[s + 1])
+        want, tol = lm_ref.kv8_attention(k, v, q[rows], [0, cu[s + 1] - cu[s]], [n], table[s:s + 1],
+                                         heads, 0, D ** -0.5, top)
+        tol = tol + 2.0 ** -70 * top + n * 2.0 ** -18 * max(2.0 ** -69 * top, 2.0 ** -126) + \
+            n * 2.0 ** -18 * want.abs() + 2.0 ** -134
+        over = (got[rows].double() - want).abs() - tol
+        assert float(over.max()) <= 0, (s, float(over.max()), float(tol.max()))
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_attention_does_not_look_past_a_row_s_tokens(ctx, D):
     """Scales of NaN on pages past the end, before the window, and on the page of a

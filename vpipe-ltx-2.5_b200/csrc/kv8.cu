@@ -885,8 +885,11 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
         m[h][e] = -INFINITY;
         l[h][e] = 0.0f;
       }
-    // O is held in units of `ref`, 1/32 of a V scale met before (0: none yet)
-    float ref = 0.0f;
+    // O is held in units of `ref`, 1/32 of a V scale met before (0: none yet), but no
+    // less than `low`: 2^-64 of the largest unit so far, so that O, 2^22 units a key at
+    // most in the largest, stays finite in any; and a normal number, as the divisions by
+    // it require
+    float ref = 0.0f, low = FLT_MIN;
 
     for (uint32_t u = 0; u < share; ++u) {
       const uint8_t* const kb = mine + stage * C::kStageBytes;
@@ -946,12 +949,16 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
         const bool masked = j0 + T > all_hi || j0 < all_lo;
         // P carries the page's V scale over ref.  ref moves when that leaves
         // [1/2, 512]: P, at most 2^kKvGrow, then stays inside f16's range and
-        // loses bits (below its normal 2^-14) only 2^13 under the row's largest
-        const bool usual = vs > 0.0f && vs <= FLT_MAX; // not zero, not NaN
+        // loses bits (below its normal 2^-14) only 2^13 under the row's largest.  A V
+        // scale under ref's lowest loses them sooner (2^-25 of that unit), and one
+        // 2^-8 of it counts as zero.
+        const bool usual = vs >= low * 0x1p-8f && vs <= FLT_MAX;   // not zero, not NaN
         float turn = 1.0f;
         if (usual && !(vs <= ref * 512.0f && vs >= ref * 0.5f)) {
-          turn = __fdividef(ref * 32.0f, vs);
-          ref = vs * 0.03125f;
+          const float to = fmaxf(vs * 0.03125f, low);
+          turn = __fdividef(ref, to);
+          ref = to;
+          low = fmaxf(low, to * 0x1p-64f);
         }
         const float ratio = usual ? __fdividef(vs, ref) : 1.0f;
         const float lift = __log2f(ratio), unlift = __fdividef(1.0f, ratio);
@@ -1037,9 +1044,9 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) l[h][e] = fmaf(sum[e], unlift, l[h][e]);
           if (!usual) {
-            // values of zero count in the sum alone; a NaN or an infinity reaches
-            // the rows that see the page
-            const float over = vs == 0.0f ? 0.0f : vs;
+            // values of zero, or so small, count in the sum alone; a NaN or an infinity
+            // reaches the rows that see the page
+            const float over = vs < low ? 0.0f : vs;
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
