@@ -688,7 +688,9 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
           w.nq = clamp_int(p.cu_q[seq + 1], w.row0, p.rows) - w.row0;
           w.key0 = clamp_int(p.cu_k[seq], 0, p.keys);
           w.nk = clamp_int(p.cu_k[seq + 1], w.key0, p.keys) - w.key0;
-          w.tok0 = max(0, slot - slot_base(w.row0, seq, T * p.tq, 1)) * (T * p.tq);
+          int tile = slot - slot_base(w.row0, seq, T * p.tq, 1);
+          if (tile < 0) w.nq = tile = 0;               // rows before the first sequence
+          w.tok0 = tile * (T * p.tq);
         }
         // keys any of the rows sees: from the first row's low to the last one's high
         const int shift = w.nk - w.nq;
