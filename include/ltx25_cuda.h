@@ -373,8 +373,8 @@ LTX_API int ltx_attention_packed(ltx_ctx* ctx, const void* q, int ldq, const voi
  * pages that nothing is appended to.
  *
  * A start, length or page outside the cache is not followed: the rows or
- * tokens that need it are left out, and the next ltx_ctx_check returns
- * LTX_E_KERNEL. */
+ * tokens that need it are left out (attention's rows with no other token are
+ * zero), and the next ltx_ctx_check returns LTX_E_KERNEL. */
 #define LTX_KV8_PAGE 64
 typedef struct {
   int8_t* k;

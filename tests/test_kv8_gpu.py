@@ -517,6 +517,35 @@ def test_places_outside_the_cache_are_not_followed(ctx):
     ctx.check()
 
 
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 16, 2), (64, 3, 3), (128, 8, 2), (256, 4, 2)])
+@pytest.mark.parametrize("lengths,seqs", [([40, 64, 1], 3), ([300, 700, 64], 3), ([30000, 130, 64], 3),
+                                          ([100, 5, 64], 400)])
+@pytest.mark.parametrize("new,window", [(1, 0), (1, 20), (3, 33)])
+def test_rows_without_a_page_are_zero(ctx, D, heads, kv_heads, lengths, seqs, new, window):
+    """Every second sequence has no page at all, or none inside its window; the others are
+    whole."""
+    import torch
+    import ltx25_b200 as L
+    lengths = [max(new, lengths[i % len(lengths)]) for i in range(seqs)]
+    cache, q, cu, table = attention_case(ctx, [new] * seqs, lengths, heads, kv_heads, D, window)
+    bad = [list(r) for r in table]
+    for s in range(0, seqs, 2):
+        first = max(0, lengths[s] - new - window + 1) // 64 if window else 0
+        for b in range(first, len(bad[s])):
+            bad[s][b] = cache.pages if b % 3 else -1
+    want, tol = expect(cache, q, cu, lengths, table, heads, window)
+    for max_len in (1, max(lengths), 10 * max(lengths)):
+        got = L.kv8_attention(ctx, cache, q, ints(cu), ints(lengths), ints(bad), heads, max_len,
+                              window=window)
+        torch.cuda.synchronize()
+        with pytest.raises(L.LtxError) as e:
+            ctx.check()
+        assert e.value.code == -6
+        got = got.view(seqs, new, -1)
+        assert torch.all(got[::2] == 0)
+        close(got[1::2], want.view(seqs, new, -1)[1::2], tol.view(seqs, new, -1)[1::2])
+
+
 def test_a_scale_that_leaves_32_bits_is_refused(ctx):
     import torch
     import ltx25_b200 as L

@@ -644,20 +644,21 @@ __device__ __forceinline__ float kv_weight(float m, float l, float top)
   return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - top);
 }
 
-// One row of a tile out of f32: columns 2 (32 e + lane) and the next of this lane.
+// One row of a tile out of f32: columns 2 (32 e + lane) and the next of this lane.  A
+// row that met no key, because it sees none or their pages are not there, has the sum
+// 0 (else its largest weight alone makes 1, or the sum is NaN) and is zero.
 template <int D>
 __device__ __forceinline__ void kv_put_row(const KvAttn& p, const KvSeq& q, int head, int rt,
                                            const float2 (&acc)[D / 64], float l)
 {
-  const int tok = rt / p.group, pos = q.len - q.n + tok, lane = (int)lane_id();
-  const bool sees = key_high(pos, q.len, 1) > key_low(pos, p.window);
+  const int tok = rt / p.group, lane = (int)lane_id();
   const float norm = 1.0f / l;
   __nv_bfloat16* dst = p.o + (size_t)(q.row0 + tok) * p.ldo +
                        (size_t)(head * p.group + rt % p.group) * D;
 #pragma unroll
   for (int e = 0; e < D / 64; ++e)
     *reinterpret_cast<uint32_t*>(dst + (e * 32 + lane) * 2) =
-        sees ? pack_bf16(acc[e].x * norm, acc[e].y * norm) : 0u;
+        l != 0.0f ? pack_bf16(acc[e].x * norm, acc[e].y * norm) : 0u;
 }
 
 // NR: groups of 8 query rows of a tile.  TEAM: a block has a tile and its warps
@@ -1138,8 +1139,7 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
         constexpr int J = D == 64 ? 4 : 8;             // tiles of a V piece
         if (whole) {
           const int tok = (row0 + r) / p.group, head = at.head * p.group + (row0 + r) % p.group;
-          const int pos = shift + tok;
-          const bool sees = key_high(pos, at.q.len, 1) > key_low(pos, p.window);
+          const bool any = l[h][e] != 0.0f;            // see kv_put_row
           const float norm = unit / l[h][e];
           __nv_bfloat16* dst = p.o + (size_t)(at.q.row0 + tok) * p.ldo + (size_t)head * D;
 #pragma unroll
@@ -1147,7 +1147,7 @@ __global__ void __launch_bounds__(KvCfg<D, NR>::kThreads, 1)
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = sees ? pack_bf16(o[h][t + i][e] * norm, o[h][t + i][2 + e] * norm) : 0u;
+              w[i] = any ? pack_bf16(o[h][t + i][e] * norm, o[h][t + i][2 + e] * norm) : 0u;
             *reinterpret_cast<uint4*>(dst + t / J * 128 + g * 2 * J + t % J * 2) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
