@@ -182,6 +182,54 @@ def test_what_a_row_does_not_see_does_not_reach_it(ctx, D, value):
     assert torch.equal(seen[~ok].isnan(), ref[~ok].isnan())
 
 
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 8, 2), (64, 3, 3), (128, 8, 2), (128, 40, 40),
+                                              (256, 4, 2)])
+@pytest.mark.parametrize("lens_q,lens_k", [
+    ([1, 15, 17, 70, 127, 129, 250, 300], None), ([400, 130], [1001, 16]), ([64], [8203]),
+    ([900, 5], [3019, 4990]), ([3] * 40, [241 + 3 * i for i in range(40)])])
+@pytest.mark.parametrize("causal,window", [(False, 0), (False, 90), (True, 0)])
+def test_the_next_sequence_leaves_no_trace(ctx, D, heads, kv_heads, lens_q, lens_k, causal, window):
+    """NaN and infinities in the keys and values right behind a sequence's last, on every
+    second sequence and behind the last of all: the others get the bits that they get
+    beside ordinary numbers."""
+    import torch
+    import ltx25_b200 as L
+    lens_k = lens_q if lens_k is None else lens_k
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, heads, kv_heads, D, 41, pad=130)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=torch.bfloat16)
+    got = []
+    for marked in (None, 0, 1):
+        a, b = k.clone(), v.clone()
+        for s in range(len(lens_k) + 1):
+            if marked is not None and (s & 1) == marked:
+                rows = slice(cu_k[s], cu_k[s + 1] if s < len(lens_k) else None)
+                n = a[rows].shape[0]
+                a[rows] = b[rows] = bad[torch.arange(n, device="cuda") % 3][:, None]
+        got.append(L.attention_packed(ctx, q, a, b, dev(cu_q), dev(cu_k), heads, kv_heads, D,
+                                      causal=causal, window=window))
+    torch.cuda.synchronize()
+    ctx.check()
+    for marked in (0, 1):
+        for s in range(1 - marked, len(lens_k), 2):
+            rows = slice(cu_q[s], cu_q[s + 1])
+            assert torch.equal(got[1 + marked][rows], got[0][rows]), (marked, s)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_the_next_sequence_costs_no_time(ctx, D):
+    """3000 rows over 5003 keys of their own, all seen, in front of a sequence of NaN."""
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu_q, cu_k = make([3000, 100], [5003, 100], 4, 4, D, 43)
+    ms = []
+    for value in (0.5, math.nan):
+        k[5003:] = v[5003:] = value
+        ms.append(best_ms(lambda: L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), 4, 4, D,
+                                                     causal=False)))
+    ctx.check()
+    assert ms[1] < 1.5 * ms[0] + 0.1, ms
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("where", ["k", "v", "both signs in v"])
 def test_what_every_row_sees_reaches_it_alone(ctx, D, where):

@@ -20,6 +20,10 @@
 //   warp 1      MMA: S = Q K^T, O += P V with P read from TMEM
 //   warp 2      takes work: finds an item's sequence and keys and hands them to
 //               the others through shared memory, one item ahead
+//   warp 3      zeroes what is not the sequence's of an item's last V tile: told by a
+//               barrier of its own (`cut`) that the tile is there, it tells `full`.
+//               The same by the MMA warp made D = 64 4 % slower, stopping the
+//               products at the last 16 keys 8 %
 //   warps 4-..  softmax, 64 score columns a thread: eight warps a query tile,
 //               two for each TMEM lane quarter, or four with a row a thread
 // An item is a CTA's query tiles of one key head.  The grid has a CTA
@@ -36,11 +40,13 @@
 // V is used as TMA lays it down, [key][64 dims] in 128-byte swizzled rows: the
 // MN-major form of the MMA's B operand, no transposed copy.
 //
-// What P multiplies must not matter where P is 0, but 0 * NaN is NaN: a key
-// tile may hold V rows that no row, or not this row, may see (the next
-// sequence's, later tokens').  A row that ends up with a NaN is therefore
-// computed again by repair_row from the keys it sees alone; a NaN that belongs
-// there comes out the same.
+// What P multiplies must not matter where P is 0, but 0 * NaN is NaN.  V rows behind
+// a sequence's last key are zeroed in shared memory before the products see them
+// (warp 3).  V rows of the sequence's own that this row, but not all of its tile, may
+// not see (later tokens', those before its window) stay: a row that ends up with a NaN
+// is computed again by repair_row from the keys it sees alone; a NaN that belongs
+// there comes out the same.  That takes 50, 145, 240 ns a row and key at head width 64,
+// 128, 256 (a warp's rows follow each other).
 //
 // Every wait is bounded; a timeout sets the context's error word and the CTA
 // drains and exits.
@@ -69,6 +75,7 @@ enum : int {
   PERR_SOFTMAX = 0x67,
   PERR_DRAIN = 0x68,
   PERR_ITEM = 0x6A,
+  PERR_CUT = 0x6B,
 };
 
 // Width 128 has two forms.  Wide: two query tiles a CTA, so that K and V are read
@@ -103,7 +110,8 @@ struct PkCfg {
   static constexpr int kMaxBytes =
       kSplit == 1 ? 0 : (kGroups * 4 + (kAlt == 2 ? 4 : 0)) * kRows * 4;
   static constexpr int kScores = kTiles * kBufs;       // score buffers
-  static constexpr int kBars = 2 * kSlots + 2 * kScores + 4 * kTiles + 8 + (kAlt == 2 ? 16 : 0);
+  static constexpr int kBars = 2 * kSlots + 2 * kScores + 4 * kTiles + 8 + 2 * kParts +
+                               (kAlt == 2 ? 16 : 0);
   static constexpr int kBarBytes = (kBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kSmem = kTiles * kQTile + kSlots * kSlot + kMaxBytes + kBarBytes + 256;
   static constexpr uint32_t kOCol = 0;                 // O_t at t * D
@@ -413,6 +421,12 @@ struct PkItem {
   int first, tiles[4];            // first key of the key tiles, their number for each query tile
 };
 
+// Keys of the sequence from the first one of key tile n - 1 on.
+__device__ __forceinline__ int pk_left(const PkItem& w, int n, int keys)
+{
+  return w.nk - w.first - (n - 1) * keys;
+}
+
 // Ask for the next CTA of the grid that has not been launched; the 16-byte answer
 // arrives in shared memory and on the barrier.
 __device__ __forceinline__ void ask_next(void* answer, uint64_t* bar)
@@ -587,7 +601,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
   uint64_t* item_empty = item_full + 2;
   uint64_t* asked = item_empty + 2;
   uint64_t* drain = asked + 1;
-  uint64_t* m_full = drain + 1;                        // [group][half][lane quarter] (kAlt 2)
+  uint64_t* cut = drain + 1;                           // [item's place][part]
+  uint64_t* m_full = cut + 2 * C::kParts;              // [group][half][lane quarter] (kAlt 2)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   uint8_t* tail = s_ring + R * C::kSlot + C::kMaxBytes + C::kBarBytes;
@@ -626,8 +641,9 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       for (int i = 0; i < 16; ++i) mbar_init(&m_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 2 + C::kGroup * T);
+      mbar_init(&item_empty[i], 3 + C::kGroup * T);
     }
+    for (int i = 0; i < 2 * C::kParts; ++i) mbar_init(&cut[i], 1);
     s_fail[0] = s_fail[1] = 0;
     mbar_init(asked, 1);
     mbar_init(drain, 1);
@@ -739,7 +755,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
   } else if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (lane == 0) {
-      uint32_t armed = 0, armed_par = 0, q_armed = 0;
+      uint32_t armed = 0, armed_par = 0, q_armed = 0, cut_armed = 0, cut_par = 0;
       int used = 0, with_keys = 0;                     // ring slots, items that have keys
       bool ok = true;
       for (int it = 0; ok; ++it) {
@@ -750,6 +766,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         if (w.head < 0) break;
         const int n = max(max(w.tiles[0], w.tiles[1]), max(w.tiles[2], w.tiles[3]));
         if (n == 0) continue;
+        const bool cuts = pk_left(w, n, kKeys) < kKeys;
         // Q's place is free once the item before has its last scores
         ok = mbar_wait(q_empty, ((uint32_t)with_keys & 1u) ^ 1u, s_abort, p.err, PERR_PRODUCER);
         if (!ok) break;
@@ -769,19 +786,26 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
             if (!ok) break;
             uint8_t* dst = s_ring + st * C::kSlot;
             const int key = w.key0 + w.first + j * kKeys;
-            mbar_arrive_expect_tx(&full[st], C::kSlot);
+            uint64_t* bar = &full[st];
+            armed |= 1u << st;
+            armed_par = (armed_par & ~(1u << st)) | (ph << st);
+            if (v && cuts && j + 1 == n) {             // warp 3 tells `full`
+              const int i = (it & 1) * C::kParts + part;
+              bar = &cut[i];
+              armed &= ~(1u << st);
+              cut_par ^= cut_armed & (1u << i);        // 0 the first time, then the other
+              cut_armed |= 1u << i;
+            }
+            mbar_arrive_expect_tx(bar, C::kSlot);
             if (v) {
               for (int a = 0; a < D / 64; ++a)
-                tma_load_3d(&tm_v, &full[st], dst + a * C::kVKeys * 128, a * 64, w.head,
+                tma_load_3d(&tm_v, bar, dst + a * C::kVKeys * 128, a * 64, w.head,
                             key + part * C::kVKeys);
             } else {
               constexpr int A = D / 64 / C::kParts;
               for (int a = 0; a < A; ++a)
-                tma_load_3d(&tm_k, &full[st], dst + a * C::kKAtom, (part * A + a) * 64, w.head,
-                            key);
+                tma_load_3d(&tm_k, bar, dst + a * C::kKAtom, (part * A + a) * 64, w.head, key);
             }
-            armed |= 1u << st;
-            armed_par = (armed_par & ~(1u << st)) | (ph << st);
           }
         };
         for (int j = 0; ok && j < min(NB, n); ++j) load(false, j);
@@ -797,6 +821,9 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       for (int st = 0; st < R; ++st)
         if (armed & (1u << st))
           mbar_wait(&full[st], (armed_par >> st) & 1u, &no_abort, p.err, PERR_DRAIN);
+      for (int i = 0; i < 2 * C::kParts; ++i)
+        if (cut_armed & (1u << i))
+          mbar_wait(&cut[i], (cut_par >> i) & 1u, &no_abort, p.err, PERR_DRAIN);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA
@@ -951,6 +978,46 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     volatile int no_abort = 0;
     mbar_wait(drain, 0, &no_abort, p.err, PERR_DRAIN);
     __syncwarp();
+  } else if (warp == 3) {
+    // ------------------------------------------------------------- cuts
+    int used = 0;                                      // ring slots
+    uint32_t seen[2] = {};                             // cuts of each place
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_abort,
+                                             p.err, PERR_CUT));
+      if (!ok) break;
+      const PkItem* w = &s_item[it & 1];
+      const int head = w->head;
+      const int n = max(max(w->tiles[0], w->tiles[1]), max(w->tiles[2], w->tiles[3]));
+      const int left = pk_left(*w, n, kKeys);
+      if (head >= 0 && n > 0) {
+        used += 2 * n * C::kParts;                     // the last V tile is its last
+        if (left < kKeys) {
+          const uint32_t parity = seen[it & 1]++ & 1u;
+#pragma unroll
+          for (int part = 0; part < C::kParts; ++part) {
+            const int st = (used - C::kParts + part) % R;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&cut[(it & 1) * C::kParts + part], parity,
+                                                         s_abort, p.err, PERR_CUT));
+            if (!ok) break;
+            // whole 128-byte rows of each 64 dims, from the first key that is not
+            // the sequence's
+            const int from = clamp_int(left - part * C::kVKeys, 0, C::kVKeys);
+            for (int i = (int)lane; i < (C::kVKeys - from) * (D / 8); i += 32)
+              *reinterpret_cast<uint4*>(s_ring + st * C::kSlot + i % (D / 8) / 8 * (C::kVKeys * 128) +
+                                        (from + i / (D / 8)) * 128 + i % 8 * 16) =
+                  make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+      if (head < 0) break;
+    }
   } else if (warp >= 4) {
     // ---------------------------------------------------------- softmax
     // Four warps a tile with a row a thread; or eight with two threads a row (hh:
