@@ -275,6 +275,22 @@ def test_calls_beyond_the_kernels_counters_are_refused(ctx):
     ctx.check()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ld", [0, 4, -8, 2 ** 31 - 1])
+def test_no_keys_at_all(ctx, D, ld):
+    """Rows without keys are zero, whatever stands for k and v."""
+    import torch
+    q, _, _, cu, _ = make([20, 1], [0, 0], 4, 2, D)
+    c, none, out = dev(cu), dev([0, 0, 0]), torch.full_like(q, 7.0)
+    rc = ctx.lib.ltx_attention_packed(
+        ctx.h, q.data_ptr(), 4 * D, None, ld, None, ld, out.data_ptr(), 4 * D, c.data_ptr(),
+        none.data_ptr(), 2, 21, 0, 4, 2, D, 1, 0, 0.125, 0)
+    assert rc == 0
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.all(out == 0)
+
+
 @pytest.mark.parametrize("D,heads,kv_heads", [(64, 8, 8), (128, 32, 4), (256, 12, 6)])
 @pytest.mark.parametrize("causal,window,prefix", [(True, 0, 0), (True, 200, 0), (True, 0, 90),
                                                   (False, 0, 0), (False, 70, 33)])

@@ -1355,11 +1355,14 @@ int pk_launch(const PackedAttention& a, int num_sms, long long base, long long c
   p.c = a.scale * 1.4426950408889634f;
   p.err = err;
   CUtensorMap mq, mk, mv;
-  // no keys at all: every row is empty and nothing loads through mk and mv
+  // no keys at all: every row is empty and nothing loads through mk and mv, which
+  // describe q then (k and v may be anything, and so may their strides)
   const bool none = a.keys == 0;
   if (!pk_encode(&mq, a.q, D, a.heads, a.rows, a.ldq, p.group, p.tq) ||
-      !pk_encode(&mk, none ? a.q : a.k, D, a.kv_heads, none ? 1 : a.keys, a.ldk, 1, C::kKeys) ||
-      !pk_encode(&mv, none ? a.q : a.v, D, a.kv_heads, none ? 1 : a.keys, a.ldv, 1, C::kVKeys))
+      !pk_encode(&mk, none ? a.q : a.k, D, a.kv_heads, none ? 1 : a.keys, none ? a.ldq : a.ldk, 1,
+                 C::kKeys) ||
+      !pk_encode(&mv, none ? a.q : a.v, D, a.kv_heads, none ? 1 : a.keys, none ? a.ldq : a.ldv, 1,
+                 C::kVKeys))
     return -1;
   if (base + count > INT_MAX || count * split > INT_MAX) return -2;
   p.by_reach = a.seqs > 1 && a.seqs <= 32 && pk_items<D, NARROW>(a) > num_sms &&
