@@ -230,6 +230,27 @@ def test_the_next_sequence_costs_no_time(ctx, D):
     assert ms[1] < 1.5 * ms[0] + 0.1, ms
 
 
+def test_rows_computed_again_over_long_keys(ctx):
+    """A NaN in the last of 300000 values: the 127 rows in front of it see all others and
+    are computed again, 32 of them by a warp, in 2.3 s.  What waits for them goes on
+    waiting (2 s is its limit for a kernel that stands still) and does the rest."""
+    import torch
+    import ltx25_b200 as L
+    D, n, m, short = 256, 128, 300000, 400
+    lens_q, lens_k = [1] * short + [n], [3] * short + [m]
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, 1, 1, D, 47)
+    v[-1, 5] = math.nan
+    out = torch.full_like(q, 7.0)
+    L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), 1, 1, D, out=out)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, 1, 1, D, True, 0, D ** -0.5)
+    check(out[:-1], want[:-1], tol[:-1], [0, short + n - 1])
+    assert torch.equal(out[-1].isnan(), want[-1].isnan()) and int(out[-1].isnan().sum()) == 1
+    ok = ~want[-1].isnan()
+    assert float(((out[-1].double() - want[-1]).abs() - tol[-1])[ok].max()) <= 0
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("where", ["k", "v", "both signs in v"])
 def test_what_every_row_sees_reaches_it_alone(ctx, D, where):

@@ -49,7 +49,8 @@
 // 128, 256 (a warp's rows follow each other).
 //
 // Every wait is bounded; a timeout sets the context's error word and the CTA
-// drains and exits.
+// drains and exits.  While a warp computes rows again (32 of 300000 keys each take 2.3 s
+// at width 256) the others' time runs from its last beat (pk_wait).
 #include <cuda.h>
 
 #include <climits>
@@ -112,7 +113,7 @@ struct PkCfg {
   static constexpr int kScores = kTiles * kBufs;       // score buffers
   static constexpr int kBars = 2 * kSlots + 2 * kScores + 4 * kTiles + 8 + 2 * kParts +
                                (kAlt == 2 ? 16 : 0);
-  static constexpr int kBarBytes = (kBars * 8 + 8 + 15) / 16 * 16;
+  static constexpr int kBarBytes = (kBars * 8 + 16 + 15) / 16 * 16;
   static constexpr int kSmem = kTiles * kQTile + kSlots * kSlot + kMaxBytes + kBarBytes + 256;
   static constexpr uint32_t kOCol = 0;                 // O_t at t * D
   static constexpr uint32_t kSCol = kTiles * D;        // tile t's buffer i at t * kBufs + i
@@ -208,14 +209,38 @@ __device__ __forceinline__ void tma_load_3d(const void* map, uint64_t* bar, void
       : "memory");
 }
 
+// A CTA's words for its waits.
+struct PkState {
+  uint32_t tmem;
+  int abort;                      // not 0: the error for which all roles leave
+  unsigned long long beat;        // when rows were last seen being computed again
+};
+
+// mbar_wait whose time runs from the last beat.  The CTA reports the error when it
+// ends: a report at each wait made captions at width 64 3 % slower.
+__device__ __forceinline__ bool pk_wait(uint64_t* bar, uint32_t parity, volatile PkState* s,
+                                        int code)
+{
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (s->abort) return false;
+    if (globaltimer_ns() - t0 > kWaitNs && globaltimer_ns() - s->beat > kWaitNs) {
+      s->abort = code;
+      return false;
+    }
+  }
+}
+
 // The NaNs among columns [col0, col0 + N) of an output row that this warp has
 // stored, looked into: a column with a NaN among its row's own values (rows
 // key0 + j of v, j in [lo, hi)) keeps it; if any is left, the row is computed again
 // from its own keys alone, in f32.  The first pass costs 1/10 of the second, so
-// that a NaN every row sees stays cheap.
+// that a NaN every row sees stays cheap.  Beats every 4096 keys.
 template <int D, int N>
-__device__ __noinline__ void repair_row(const PkParams& p, int row, int head, int kvh, int key0,
-                                        int lo, int hi, int col0)
+__device__ __noinline__ void repair_row(const PkParams& p, volatile PkState* s, int row, int head,
+                                        int kvh, int key0, int lo, int hi, int col0)
 {
   constexpr int W = N / 32;                       // columns of a lane, 2 or 4
   const int lane = (int)lane_id();
@@ -229,6 +254,7 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
   }
   bool found[W] = {};
   for (int j = lo; j < hi && __any_sync(0xffffffffu, open); j += 16) {
+    if (((j - lo) & 4095) == 0) s->beat = globaltimer_ns();
     open = false;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -250,6 +276,7 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
   float m = -INFINITY, l = 0.0f, acc[W];
   for (int e = 0; e < W; ++e) acc[e] = 0.0f;
   for (int j0 = lo; j0 < hi; j0 += 32) {
+    if (((j0 - lo) & 4095) == 0) s->beat = globaltimer_ns();
     const int n = min(32, hi - j0);
     const uint4* k = reinterpret_cast<const uint4*>(
         p.k + (size_t)(key0 + j0 + min(lane, n - 1)) * p.ldk + (size_t)kvh * D);
@@ -264,13 +291,13 @@ __device__ __noinline__ void repair_row(const PkParams& p, int row, int head, in
         dot = fmaf(__uint_as_float(aw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), dot);
       }
     }
-    const float s = lane < n ? dot * p.c : -INFINITY;
-    float mx = s;
+    const float score = lane < n ? dot * p.c : -INFINITY;
+    float mx = score;
     for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
     const float m_new = fmaxf(m, mx);
     const float r = m_new == -INFINITY ? 0.0f : m_new;
     const float f = m == -INFINITY ? 0.0f : exp2f(m - r);
-    const float pj = lane < n ? exp2f(s - r) : 0.0f;
+    const float pj = lane < n ? exp2f(score - r) : 0.0f;
     m = m_new;
     l = l * f + pj;                               // this lane's share
     for (int e = 0; e < W; ++e) acc[e] *= f;
@@ -480,8 +507,8 @@ __device__ __forceinline__ uint32_t pk_part(int row, int c)
 // in the CTAs' order.  A thread has 4 columns at a time, a warp whole rows or 128
 // columns, and asks for 4 parts at once.
 template <int D, int T, int S>
-__device__ __forceinline__ void pk_join(const PkParams& p, const PkItem& w, uint32_t parts,
-                                        uint32_t sums, int tid, int threads)
+__device__ __forceinline__ void pk_join(const PkParams& p, volatile PkState* s, const PkItem& w,
+                                        uint32_t parts, uint32_t sums, int tid, int threads)
 {
   constexpr int kPieces = D / 4, kSpan = D < 128 ? D : 128;
   constexpr int kBatch = S < 4 ? S : 4, kAhead = 4 / kBatch;
@@ -560,7 +587,7 @@ __device__ __forceinline__ void pk_join(const PkParams& p, const PkItem& w, uint
       while (bad != 0) {
         const int src = __ffs((int)bad) - 1;
         bad &= kPieces < 32 ? ~(((1u << (kPieces & 31)) - 1u) << (src / kPieces * kPieces)) : 0u;
-        repair_row<D, kSpan>(p, __shfl_sync(0xffffffffu, row, src),
+        repair_row<D, kSpan>(p, s, __shfl_sync(0xffffffffu, row, src),
                              __shfl_sync(0xffffffffu, head, src), w.head, w.key0,
                              __shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src),
                              __shfl_sync(0xffffffffu, c * 4 / kSpan * kSpan, src));
@@ -603,8 +630,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
   uint64_t* drain = asked + 1;
   uint64_t* cut = drain + 1;                           // [item's place][part]
   uint64_t* m_full = cut + 2 * C::kParts;              // [group][half][lane quarter] (kAlt 2)
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + C::kBars);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  volatile PkState* s_state = reinterpret_cast<volatile PkState*>(bars + C::kBars);
   uint8_t* tail = s_ring + R * C::kSlot + C::kMaxBytes + C::kBarBytes;
   uint8_t* s_answer = tail;                            // 16 bytes
   volatile int* s_fail = reinterpret_cast<volatile int*>(tail + 16);    // one a query tile
@@ -647,7 +673,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     s_fail[0] = s_fail[1] = 0;
     mbar_init(asked, 1);
     mbar_init(drain, 1);
-    *s_abort = 0;
+    s_state->abort = 0;
+    s_state->beat = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -656,13 +683,13 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   if (warp == 1) {
-    tmem_alloc(s_tmem, 512);
+    tmem_alloc(const_cast<uint32_t*>(&s_state->tmem), 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *s_tmem;
+  const uint32_t tmem = s_state->tmem;
   pdl_wait();
   pdl_trigger();
 
@@ -730,8 +757,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
           w.first += from * kKeys;
         }
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u,
-                                             s_abort, p.err, PERR_ITEM));
+      ok = __all_sync(0xffffffffu, pk_wait(&item_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u,
+                                           s_state, PERR_ITEM));
       if (ok && lane == 0) {
         s_item[it & 1] = w;
         mbar_arrive(&item_full[it & 1]);
@@ -759,7 +786,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       int used = 0, with_keys = 0;                     // ring slots, items that have keys
       bool ok = true;
       for (int it = 0; ok; ++it) {
-        ok = mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_abort, p.err, PERR_PRODUCER);
+        ok = pk_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_state, PERR_PRODUCER);
         if (!ok) break;
         const PkItem w = s_item[it & 1];
         mbar_arrive(&item_empty[it & 1]);
@@ -768,7 +795,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         if (n == 0) continue;
         const bool cuts = pk_left(w, n, kKeys) < kKeys;
         // Q's place is free once the item before has its last scores
-        ok = mbar_wait(q_empty, ((uint32_t)with_keys & 1u) ^ 1u, s_abort, p.err, PERR_PRODUCER);
+        ok = pk_wait(q_empty, ((uint32_t)with_keys & 1u) ^ 1u, s_state, PERR_PRODUCER);
         if (!ok) break;
         mbar_arrive_expect_tx(q_full, (uint32_t)(T * (D / 64) * p.group * p.tq * 128));
         for (int t = 0; t < T; ++t)
@@ -782,7 +809,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
           for (int part = 0; ok && part < C::kParts; ++part, ++used) {
             const int st = used % R;
             const uint32_t ph = (uint32_t)(used / R) & 1u;
-            ok = mbar_wait(&empty[st], ph ^ 1u, s_abort, p.err, PERR_PRODUCER);
+            ok = pk_wait(&empty[st], ph ^ 1u, s_state, PERR_PRODUCER);
             if (!ok) break;
             uint8_t* dst = s_ring + st * C::kSlot;
             const int key = w.key0 + w.first + j * kKeys;
@@ -832,7 +859,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     const uint32_t lead = elect_lane();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, s_abort, p.err, PERR_MMA)) != 0;
+      return __all_sync(0xffffffffu, pk_wait(bar, parity, s_state, PERR_MMA)) != 0;
     };
     // a place in the ring of slots and the parity of its round
     struct Ring {
@@ -984,8 +1011,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
     uint32_t seen[2] = {};                             // cuts of each place
     bool ok = true;
     for (int it = 0; ok; ++it) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_abort,
-                                             p.err, PERR_CUT));
+      ok = __all_sync(0xffffffffu, pk_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u, s_state,
+                                           PERR_CUT));
       if (!ok) break;
       const PkItem* w = &s_item[it & 1];
       const int head = w->head;
@@ -998,14 +1025,15 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
 #pragma unroll
           for (int part = 0; part < C::kParts; ++part) {
             const int st = (used - C::kParts + part) % R;
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&cut[(it & 1) * C::kParts + part], parity,
-                                                         s_abort, p.err, PERR_CUT));
+            ok = ok && __all_sync(0xffffffffu, pk_wait(&cut[(it & 1) * C::kParts + part], parity,
+                                                       s_state, PERR_CUT));
             if (!ok) break;
             // whole 128-byte rows of each 64 dims, from the first key that is not
             // the sequence's
             const int from = clamp_int(left - part * C::kVKeys, 0, C::kVKeys);
             for (int i = (int)lane; i < (C::kVKeys - from) * (D / 8); i += 32)
-              *reinterpret_cast<uint4*>(s_ring + st * C::kSlot + i % (D / 8) / 8 * (C::kVKeys * 128) +
+              *reinterpret_cast<uint4*>(s_ring + st * C::kSlot +
+                                        i % (D / 8) / 8 * (C::kVKeys * 128) +
                                         (from + i / (D / 8)) * 128 + i % 8 * 16) =
                   make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1042,8 +1070,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       // Two warps a row meet at barriers, so all warps of a tile agree on going on:
       // a wait that failed is told before one, and their number in an item is the
       // same for all.
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u,
-                                                   s_abort, p.err, PERR_SOFTMAX));
+      ok = __all_sync(0xffffffffu, ok && pk_wait(&item_full[it & 1], (uint32_t)(it >> 1) & 1u,
+                                                 s_state, PERR_SOFTMAX));
       if (kSplit * kAlt == 1) {
         if (!ok) break;
       } else {
@@ -1076,8 +1104,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         const uint32_t at = step + (uint32_t)i;        // this score tile
         const int sb = t * NB + (int)(at % (uint32_t)NB);
         const uint32_t scol = tmem + lane_base + C::kSCol + (uint32_t)(sb * kKeys);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&s_full[sb], (at / (uint32_t)NB) & 1u, s_abort,
-                                                     p.err, PERR_SOFTMAX));
+        ok = __all_sync(0xffffffffu, ok && pk_wait(&s_full[sb], (at / (uint32_t)NB) & 1u, s_state,
+                                                   PERR_SOFTMAX));
         uint32_t a[32], b[32];
         tc_fence_after();
         tmem_ld32(scol + (uint32_t)(hh * 64), a);
@@ -1120,8 +1148,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
             m_old = -INFINITY;
           } else {
             ok = __all_sync(0xffffffffu,
-                            ok && mbar_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
-                                            ((at - 1u) >> 1) & 1u, s_abort, p.err, PERR_SOFTMAX));
+                            ok && pk_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
+                                          ((at - 1u) >> 1) & 1u, s_state, PERR_SOFTMAX));
             m_old = s_m[alt ^ 1][hh][r];
           }
         }
@@ -1159,9 +1187,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
           // All of O but this key tile's part.  Of the barrier's two rounds back the
           // P V at - 3 is done (these scores came after it), so the parity is plain;
           // with one barrier P V at - 2, under way or done, would leave it open.
-          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * t + (int)((at - 1u) & 1u)],
-                                                 ((at - 1u) >> 1) & 1u, s_abort, p.err,
-                                                 PERR_SOFTMAX));
+          ok = __all_sync(0xffffffffu, pk_wait(&o_done[2 * t + (int)((at - 1u) & 1u)],
+                                               ((at - 1u) >> 1) & 1u, s_state, PERR_SOFTMAX));
           if (ok) {
             tc_fence_after();
 #pragma unroll
@@ -1187,8 +1214,8 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         const uint32_t end = step + (uint32_t)nt - 1u;
         if ((int)(end & 1u) != alt) {
           ok = __all_sync(0xffffffffu,
-                          ok && mbar_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
-                                          (end >> 1) & 1u, s_abort, p.err, PERR_SOFTMAX));
+                          ok && pk_wait(&m_full[((alt ^ 1) * 2 + hh) * 4 + quarter],
+                                        (end >> 1) & 1u, s_state, PERR_SOFTMAX));
           m_end = s_m[alt ^ 1][hh][r];
         }
         if (m_run != m_end) l_row *= fast_exp2(m_run - m_end);
@@ -1213,15 +1240,15 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       const bool stores = kAlt == 1 || (nt > 0 ? (int)((step - 1u) & 1u) != alt : alt == 0);
       if (nt > 0) {
         if (stores)
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_last[t], closed & 1u, s_abort, p.err,
-                                                       PERR_SOFTMAX));
+          ok = __all_sync(0xffffffffu, ok && pk_wait(&o_last[t], closed & 1u, s_state,
+                                                     PERR_SOFTMAX));
         ++closed;
       }
       if constexpr (SPLIT) {
         // O and (maximum, sum) to this CTA's shared memory, once the products of all
         // query tiles are through with it; 16-byte pieces in turn against bank conflicts
         constexpr int kCols = D / kSplit;
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(drain, 0, s_abort, p.err, PERR_SOFTMAX));
+        ok = __all_sync(0xffffffffu, ok && pk_wait(drain, 0, s_state, PERR_SOFTMAX));
         if (ok && stores) {
           tc_fence_after();
 #pragma unroll
@@ -1260,7 +1287,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
         while (bad != 0) {
           const int src = __ffs((int)bad) - 1;
           bad &= bad - 1;
-          repair_row<D, kCols>(p, __shfl_sync(0xffffffffu, row, src),
+          repair_row<D, kCols>(p, s_state, __shfl_sync(0xffffffffu, row, src),
                                __shfl_sync(0xffffffffu, head, src), w->head, w->key0,
                                __shfl_sync(0xffffffffu, lo, src),
                                __shfl_sync(0xffffffffu, hi, src), hh * kCols);
@@ -1274,9 +1301,9 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
       if (joins) {
         const uint32_t parts = smem_u32(s_ring), sums = smem_u32(s_q);
         const int tid = (int)threadIdx.x - 128, threads = C::kThreads - 128;
-        if (p.split == 2) pk_join<D, T, 2>(p, s_item[0], parts, sums, tid, threads);
-        else if (p.split == 4) pk_join<D, T, 4>(p, s_item[0], parts, sums, tid, threads);
-        else pk_join<D, T, 8>(p, s_item[0], parts, sums, tid, threads);
+        if (p.split == 2) pk_join<D, T, 2>(p, s_state, s_item[0], parts, sums, tid, threads);
+        else if (p.split == 4) pk_join<D, T, 4>(p, s_state, s_item[0], parts, sums, tid, threads);
+        else pk_join<D, T, 8>(p, s_state, s_item[0], parts, sums, tid, threads);
       }
     }
   }
@@ -1287,6 +1314,7 @@ __global__ void __launch_bounds__(PkCfg<D, NARROW>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0 && s_state->abort != 0) atomicCAS(p.err, 0, s_state->abort);
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
