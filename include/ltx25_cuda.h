@@ -344,7 +344,9 @@ LTX_API int ltx_attention(ltx_ctx* ctx, const void* q, int ldq, const void* k,
  * h / (heads / kv_heads); head_dim 64, 128 or 256; at most 128 query heads a
  * key/value head.  Sequence offsets, lengths and page tables are DEVICE
  * int32 arrays: the host does not read them, the kernels bound every value by
- * the sizes given here. */
+ * the sizes given here.  Sums are f32: finite inputs give the
+ * formula's finite results where head_dim * max|q| * max|k|, that times scale,
+ * and max|v| times the keys stay below 1e36. */
 
 /* Attention over packed prompts of different lengths.  Sequence s has the
  * query rows [cu_q[s], cu_q[s+1]) of q and o (`rows` rows) and the keys
@@ -393,7 +395,8 @@ typedef struct {
  * larger and the page holds tokens of the sequence already
  * (starts[s] % LTX_KV8_PAGE != 0, first page).  New codes are
  * rint(x / scale); codes the page held are brought to a grown scale as
- * rint(code * old / new).  A NaN or infinity makes the scale of its page and
+ * rint(code * old / new).  (Normal values appended one token at a time end 0.38
+ * of the scale off, rms, against 0.29 appended at once.)  A NaN or infinity makes the scale of its page and
  * head NaN.  A page that gets tokens stands once in the table's used columns,
  * for one sequence. */
 LTX_API int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,

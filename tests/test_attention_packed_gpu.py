@@ -230,6 +230,24 @@ def test_the_next_sequence_costs_no_time(ctx, D):
     assert ms[1] < 1.5 * ms[0] + 0.1, ms
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens_q,lens_k", [([500], [500]), ([30], [9000])])
+def test_the_largest_finite_numbers(ctx, D, lens_q, lens_k):
+    """Up to 1e36: max|v| times the keys, D max|q| max|k|."""
+    import torch
+    import ltx25_b200 as L
+    q, k, v, cu_q, cu_k = make(lens_q, lens_k, 4, 2, D, 51, 3.0)
+    e = math.floor(math.log2(1e36 / (D * float(q.abs().max()) * float(k.abs().max()))) / 2)
+    q, k = q * 2.0 ** e, k * 2.0 ** e
+    v = v * 2.0 ** math.floor(math.log2(1e36 / (lens_k[0] * float(v.abs().max()))))
+    scale = D ** -0.5 * 2.0 ** (-2 * e)
+    got = L.attention_packed(ctx, q, k, v, dev(cu_q), dev(cu_k), 4, 2, D, scale=scale)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.attention_packed(q, k, v, cu_q, cu_k, 4, 2, D, True, 0, scale)
+    check(got, want, tol, cu_q)
+
+
 def test_rows_computed_again_over_long_keys(ctx):
     """A NaN in the last of 300000 values: the 127 rows in front of it see all others and
     are computed again, 32 of them by a warp, in 2.3 s.  What waits for them goes on

@@ -347,6 +347,28 @@ def test_attention_over_value_scales_at_the_ends_of_the_range(ctx, D, exps, new,
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths,max_len", [([300, 40], 300), ([9000, 700], 9000)])
+def test_attention_of_the_largest_finite_numbers(ctx, D, lengths, max_len):
+    """Up to 1e36: max|v| times the keys, D max|q| max|k|."""
+    import torch
+    import ltx25_b200 as L
+    cache, q, cu, table = attention_case(ctx, [2, 1], lengths, 4, 2, D, 0, 3.0)
+    kmax, vmax = (127 * float(s.double().max()) for s in (cache.k_scale, cache.v_scale))
+    e = math.floor(math.log2(1e36 / (D * float(q.abs().max()) * kmax)) / 2)
+    q, scale = q * 2.0 ** e, D ** -0.5 * 2.0 ** (-2 * e)
+    cache = L.KV8Cache(cache.k, cache.v, cache.k_scale * 2.0 ** e, cache.v_scale *
+                       2.0 ** math.floor(math.log2(1e36 / (lengths[0] * vmax))))
+    got = L.kv8_attention(ctx, cache, q, ints(cu), ints(lengths), ints(table), 4, max_len,
+                          scale=scale)
+    torch.cuda.synchronize()
+    ctx.check()
+    want, tol = lm_ref.kv8_attention(values(cache.k, cache.k_scale),
+                                     values(cache.v, cache.v_scale), q, cu, lengths, table, 4, 0,
+                                     scale, float(cache.v_scale.double().max()))
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_attention_does_not_look_past_a_row_s_tokens(ctx, D):
     """Scales of NaN on pages past the end, before the window, and on the page of a
     later new token; codes behind the last token of a page."""

@@ -40,6 +40,10 @@
 // V is used as TMA lays it down, [key][64 dims] in 128-byte swizzled rows: the
 // MN-major form of the MMA's B operand, no transposed copy.
 //
+// P is rounded to bf16, as the MMA takes it beside a bf16 V, while its sum stays f32:
+// 2^-8 of a term and independent from term to term, so the listed calls are off by
+// 0.0019 to 0.0023 rms against 64 bits, where rounding the result alone makes 0.0016.
+//
 // What P multiplies must not matter where P is 0, but 0 * NaN is NaN.  V rows behind
 // a sequence's last key are zeroed in shared memory before the products see them
 // (warp 3).  V rows of the sequence's own that this row, but not all of its tile, may
@@ -86,6 +90,12 @@ enum : int {
 // 128 keys; half the rows an item.  Under the power cap the wide form runs long
 // prompts faster all the same (528 against 544 us, 8192 tokens, at 1.69 against
 // 1.55 GHz), so the narrow one takes calls whose wide items would not fill the SMs.
+// That rule is plain, not the best where wide items fill the SMs once and a little,
+// since wide items share no keys.  32/8 heads, one sequence, us (wide / narrow):
+//   new tokens on 8000       1100       1151       1153       1300       1600       2300
+//                         140 / 132  141 / 134  263 / 149  262 / 185  270 / 205  294 / 302
+//   prompts                  1300       2000       2400       4000       8192
+//                        32.4 / 28.4  51.6 / 46.5  68 / 59   141 / 127  483 / 507
 template <int D, bool NARROW>
 struct PkCfg {
   static_assert(D == 128 || !NARROW, "forms");
@@ -1445,6 +1455,11 @@ int pk_clusters(int n)
 //   new tokens, keys before      500           2000          8000          32000
 //   16                        9.6 /  8.6   19.1 /  9.8   56.1 / 15.9   204.3 / 35.6
 //   64                       11.1 / 10.7   19.8 / 12.4   58.0 / 23.1   206.7 / 61.8
+// and, 16 tokens, 32/8 heads of 64:
+//                            12.3 /  9.4   33.8 / 11.9    116 / 21.7     449 / 60.8
+// 16/8 heads of 256:         12.0 / 12.0   27.7 / 11.2   89.0 / 20.6     333 / 52.8
+// (kStep is a whole item's; at width 64 one with few rows, one query tile of four,
+// takes less: 115 us for the 8000 keys against 136 for 64 tokens.)
 template <int D, bool NARROW>
 int pk_split(long long items, float alone, float start, int num_sms)
 {

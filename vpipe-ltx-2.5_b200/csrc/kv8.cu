@@ -130,7 +130,10 @@ __device__ __forceinline__ uint32_t joined_scale(uint32_t most, uint32_t was, bo
 }
 
 // The page's own codes, brought to a grown scale: c * was / now, a quotient of 15
-// by 8 bits, decided by the correctly rounded f32 division.
+// by 8 bits, decided by the correctly rounded f32 division.  Each growth rounds them
+// anew.  A page of 64 normal values a column filled token by token is off by 0.38 of
+// its scale rms (2.1 at most of 64k values), filled at once by 0.29 (0.5); where the
+// values grow threefold along the page by 0.57 (2.7), 64-fold by 0.71 (2.2).
 __device__ __forceinline__ void rescale_codes(int8_t* codes, int count4, uint32_t was, uint32_t now,
                                               int at, int step)
 {
@@ -159,7 +162,8 @@ __device__ __forceinline__ unsigned long long fmul2(unsigned long long a, unsign
 //   adding 1.5 * 2^23 - 1.5 * 2^12 rounds to the nearest integer, ties to even,
 //   and leaves the code in the sum's low byte.
 // Two values at a time (a value at a time, with the two last additions apart and the
-// old scale read for new pages too, 90 MB of prompts took 25 us, now 18).  1 / s may not be finite for a tiny s: x goes through 2^64 / (2^64 s) there.
+// old scale read for new pages too, 90 MB of prompts took 25 us, now 18).  1 / s may
+// not be finite for a tiny s: x goes through 2^64 / (2^64 s) there.
 struct KvCoder {
   unsigned long long inv;
   float mul;                      // 1, or 2^64 ahead of inv
@@ -370,7 +374,9 @@ __global__ void __launch_bounds__(kAppendThreads)
 // O^T = V^T P^T, on warp MMAs with f32 sums (m16n8k16, f16 operands): 16 keys or
 // 16 output columns by 8 query rows, since a decoded token has no more rows than
 // query heads share a key head.  Against 16 query rows in the M place that halves
-// the MMAs, the exponentials and the registers.  P rounds at 2^-11; q's 8 bits are
+// the MMAs, the exponentials and the registers.  f16 is what the MMA takes beside the
+// codes: P rounds at 2^-11, under the result's own bf16 rounding of 2^-8 (against 64
+// bits the listed calls are off by 0.00165 rms, the f32 form by the same); q's 8 bits are
 // exact once its row is brought near 2^8 by a power of two.  Measured on 131072
 // tokens, 8 key heads of 128 under 4 query heads each: 48.8 us for 268 MB (5.5 TB/s),
 // 739 warp instructions a stage (903 that way), 55 % of the issue slots, tensor pipe
@@ -1425,7 +1431,18 @@ int kv_attn_launch(const Kv8Attention& a, int num_sms, int* err, cudaStream_t s)
   //   8 tiles     6.2 /  8.2    9.6 /  9.2   15.6 /  9.4   24.1 / 10.0
   //   32          6.6 / 11.8   10.1 / 12.3   16.2 / 14.4   24.9 / 16.8
   //   64          6.7 / 11.0   10.4 / 15.3   16.8 / 19.4   25.6 / 24.4
-  // and not beyond 6 stages a warp, since lengths may be anything up to max_len.
+  // and not beyond 6 stages a warp, since lengths may be anything up to max_len.  The same
+  // numbers serve the other widths and tiles of 16 rows (us for 300, 1000, 2000, 4000
+  // tokens, TEAM / equal runs, * the rule's choice):
+  //   width  64,  8 tiles    5.4* 7.9   7.2*  9.0   9.5* 10.1  15.1  10.3*
+  //              64          5.9*10.5   7.9* 11.5  10.3* 13.9  16.0* 17.1
+  //   width 256,  8          8.3* 9.2  15.9   9.4* 27.2  10.5* 50.0  12.3*
+  //              64          8.9*12.6  16.6  15.8* 28.5  22.1* 51.9  33.1*
+  //   128, 16 rows, 8       10.1*13.0  14.3  13.5* 21.7  13.9* 36.5  14.9*
+  //              32         10.3*26.6  14.5* 28.8  21.9  31.1* 36.6  34.4*
+  //              64         10.4*15.1  14.6* 19.8  22.2  25.5* 37.5  33.1*
+  // Equal runs of 32 tiles of 16 rows pay for a join of a warp a row that is slow for so
+  // many; there and with 64 the rule gives up on TEAM too early at 2000 tokens.
   const long long used = p.rows == p.seqs ? (long long)p.seqs * ((p.group + 8 * NR - 1) / (8 * NR))
                                           : slots;                  // slots with rows
   const long long rounds = (units + C::kWarps - 1) / C::kWarps;
