@@ -236,7 +236,9 @@ __device__ __forceinline__ bool pk_wait(uint64_t* bar, uint32_t parity, volatile
   while (true) {
     if (mbar_try_wait(bar, parity)) return true;
     if (s->abort) return false;
-    if (globaltimer_ns() - t0 > kWaitNs && globaltimer_ns() - s->beat > kWaitNs) {
+    // (signed: a beat may come between the two reads)
+    if (globaltimer_ns() - t0 > kWaitNs &&
+        (long long)(globaltimer_ns() - s->beat) > (long long)kWaitNs) {
       s->abort = code;
       return false;
     }
