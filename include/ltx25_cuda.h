@@ -396,8 +396,8 @@ typedef struct {
  * (starts[s] % LTX_KV8_PAGE != 0, first page).  New codes are
  * rint(x / scale); codes the page held are brought to a grown scale as
  * rint(code * old / new).  (Normal values appended one token at a time end 0.38
- * of the scale off, rms, against 0.29 appended at once.)  A NaN or infinity makes the scale of its page and
- * head NaN.  A page that gets tokens stands once in the table's used columns,
+ * of the scale off, rms, against 0.29 appended at once.)  A NaN or infinity
+ * makes the scale of its page and head NaN.  A page that gets tokens stands once in the table's used columns,
  * for one sequence. */
 LTX_API int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,
                            const void* v, int ldv, const int32_t* cu, const int32_t* starts,
