@@ -397,8 +397,8 @@ typedef struct {
  * rint(x / scale); codes the page held are brought to a grown scale as
  * rint(code * old / new).  (Normal values appended one token at a time end 0.38
  * of the scale off, rms, against 0.29 appended at once.)  A NaN or infinity
- * makes the scale of its page and head NaN.  A page that gets tokens stands once in the table's used columns,
- * for one sequence. */
+ * makes the scale of its page and head NaN.  A page that gets tokens stands
+ * once in the table's used columns, for one sequence. */
 LTX_API int ltx_kv8_append(ltx_ctx* ctx, const ltx_kv8_cache* cache, const void* k, int ldk,
                            const void* v, int ldv, const int32_t* cu, const int32_t* starts,
                            const int32_t* table, int table_ld, int seqs, int rows, void* stream);

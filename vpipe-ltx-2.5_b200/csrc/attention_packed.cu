@@ -41,7 +41,7 @@
 // MN-major form of the MMA's B operand, no transposed copy.
 //
 // P is rounded to bf16, as the MMA takes it beside a bf16 V, while its sum stays f32:
-// 2^-8 of a term and independent from term to term, so the listed calls are off by
+// 2^-8 of a term and independent from term to term, so prompts of normal values are off by
 // 0.0019 to 0.0023 rms against 64 bits, where rounding the result alone makes 0.0016.
 //
 // What P multiplies must not matter where P is 0, but 0 * NaN is NaN.  V rows behind

@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kAppendThreads)
 // query heads share a key head.  Against 16 query rows in the M place that halves
 // the MMAs, the exponentials and the registers.  f16 is what the MMA takes beside the
 // codes: P rounds at 2^-11, under the result's own bf16 rounding of 2^-8 (against 64
-// bits the listed calls are off by 0.00165 rms, the f32 form by the same); q's 8 bits are
+// bits normal values are off by 0.00165 rms, the f32 form by the same); q's 8 bits are
 // exact once its row is brought near 2^8 by a power of two.  Measured on 131072
 // tokens, 8 key heads of 128 under 4 query heads each: 48.8 us for 268 MB (5.5 TB/s),
 // 739 warp instructions a stage (903 that way), 55 % of the issue slots, tensor pipe
